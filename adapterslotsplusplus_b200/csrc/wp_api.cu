@@ -2016,4 +2016,177 @@ int wp_read_bridge_kernel(wp_handle* h, float* out, int32_t cap, int32_t* count)
   return WP_OK;
 }
 
+// ---- operators around the LoRA projections -------------------------------------
+
+static int check_seqs(wp_handle* h, const char* what, const wp::Kv4Args& a, int32_t head_dim, int32_t dtype) {
+  if (!dtype16(dtype)) return fail(h, WP_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
+  if (head_dim != 64 && head_dim != 128) return fail(h, WP_ERR_INVALID, "%s: head_dim must be 64 or 128, got %d", what, head_dim);
+  if (a.kv_heads < 1 || a.kv_heads > 65535 || a.num_seqs < 0 || a.tokens < 0 || a.num_pages < 0 || a.page_tiles < 1 ||
+      a.table_ld < 0)
+    return fail(h, WP_ERR_INVALID, "%s: bad sizes", what);
+  if (a.num_seqs > 0 && (!a.table || !a.lens || !a.pages)) return fail(h, WP_ERR_INVALID, "%s: NULL pages, table or lengths", what);
+  if (!al16(a.pages)) return fail(h, WP_ERR_INVALID, "%s: pages must be 16-byte aligned", what);
+  if (!a.cu && a.tokens != a.num_seqs) return fail(h, WP_ERR_INVALID, "%s: without offsets every sequence has one token", what);
+  return WP_OK;
+}
+
+// Rows of head_dim contiguous elements that 16-byte loads can take.
+static bool rows_ok(const void* p, int64_t ts, int64_t hs) { return p && al16(p) && ts % 8 == 0 && hs % 8 == 0; }
+
+int64_t wp_kv4_tile_bytes(int32_t head_dim) {
+  return head_dim == 64 || head_dim == 128 ? wp::kv4_tile_bytes(head_dim) : 0;
+}
+
+int wp_kv4_append(wp_handle* h, void* pages, int32_t num_pages, int32_t page_size, const void* k, int64_t k_ts,
+                  int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, const int32_t* table, int64_t table_ld,
+                  const int32_t* lens, const int32_t* cu, int32_t num_seqs, int32_t tokens, int32_t kv_heads,
+                  int32_t head_dim, int32_t dtype, void* stream) {
+  if (!h) return fail(nullptr, WP_ERR_INVALID, "kv4_append: NULL handle");
+  wp::Kv4Args a{};
+  a.pages = static_cast<uint8_t*>(pages);
+  a.table = table;
+  a.lens = lens;
+  a.cu = cu;
+  a.table_ld = table_ld;
+  a.num_pages = num_pages;
+  a.page_tiles = page_size / wp::kKv4Tile;
+  a.num_seqs = num_seqs;
+  a.tokens = tokens;
+  a.kv_heads = kv_heads;
+  a.k = const_cast<void*>(k);
+  a.v = const_cast<void*>(v);
+  a.k_ts = k_ts;
+  a.k_hs = k_hs;
+  a.v_ts = v_ts;
+  a.v_hs = v_hs;
+  a.err = h->d_err;
+  if (page_size % wp::kKv4Tile) return fail(h, WP_ERR_INVALID, "kv4_append: page_size must be a multiple of 16");
+  if (int rc = check_seqs(h, "kv4_append", a, head_dim, dtype)) return rc;
+  if (num_seqs == 0 || tokens == 0) return WP_OK;
+  if (!rows_ok(k, k_ts, k_hs) || !rows_ok(v, v_ts, v_hs))
+    return fail(h, WP_ERR_INVALID, "kv4_append: k and v need 16-byte aligned rows (strides in multiples of 8 elements)");
+  DeviceGuard dg(h->device);
+  cudaError_t e = wp::launch_kv4_append(dtype, head_dim, a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(h, WP_ERR_CUDA, "kv4_append launch: %s", cudaGetErrorString(e));
+  ++h->launches;
+  return WP_OK;
+}
+
+int wp_kv4_read(wp_handle* h, void* k, void* v, const void* pages, int32_t num_pages, int32_t page_size,
+                const int32_t* table, int64_t table_ld, const int32_t* lens, const int32_t* cu, int32_t num_seqs,
+                int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t dtype, void* stream) {
+  if (!h) return fail(nullptr, WP_ERR_INVALID, "kv4_read: NULL handle");
+  wp::Kv4Args a{};
+  a.pages = static_cast<uint8_t*>(const_cast<void*>(pages));
+  a.table = table;
+  a.lens = lens;
+  a.cu = cu;
+  a.table_ld = table_ld;
+  a.num_pages = num_pages;
+  a.page_tiles = page_size / wp::kKv4Tile;
+  a.num_seqs = num_seqs;
+  a.tokens = tokens;
+  a.kv_heads = kv_heads;
+  a.k = k;
+  a.v = v;
+  a.err = h->d_err;
+  if (page_size % wp::kKv4Tile) return fail(h, WP_ERR_INVALID, "kv4_read: page_size must be a multiple of 16");
+  if (int rc = check_seqs(h, "kv4_read", a, head_dim, dtype)) return rc;
+  if (num_seqs == 0 || tokens == 0) return WP_OK;
+  if (!k || !v || !al16(k) || !al16(v)) return fail(h, WP_ERR_INVALID, "kv4_read: k and v must be 16-byte aligned");
+  DeviceGuard dg(h->device);
+  cudaError_t e = wp::launch_kv4_read(dtype, head_dim, a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(h, WP_ERR_CUDA, "kv4_read launch: %s", cudaGetErrorString(e));
+  ++h->launches;
+  return WP_OK;
+}
+
+int64_t wp_kv4_attention_workspace(wp_handle* h, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_q,
+                                   int32_t dtype) {
+  if (!h || kv_heads < 1 || heads < kv_heads || (head_dim != 64 && head_dim != 128) || !dtype16(dtype)) return -1;
+  DeviceGuard dg(h->device);
+  return wp::kv4_attention_workspace(dtype, head_dim, heads / kv_heads, std::max(max_q, 1), h->num_sms);
+}
+
+int wp_kv4_attention(wp_handle* h, void* out, float* lse, const void* q, int64_t q_ts, int64_t q_hs, const void* pages,
+                     int32_t num_pages, int32_t page_size, const int32_t* table, int64_t table_ld, const int32_t* lens,
+                     const int32_t* cu, int32_t num_seqs, int32_t max_q, int32_t tokens, int32_t heads,
+                     int32_t kv_heads, int32_t head_dim, float scale, int32_t dtype, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+  if (!h) return fail(nullptr, WP_ERR_INVALID, "kv4_attention: NULL handle");
+  wp::Kv4Args a{};
+  a.pages = static_cast<uint8_t*>(const_cast<void*>(pages));
+  a.table = table;
+  a.lens = lens;
+  a.cu = cu;
+  a.table_ld = table_ld;
+  a.num_pages = num_pages;
+  a.page_tiles = page_size / wp::kKv4Tile;
+  a.num_seqs = num_seqs;
+  a.tokens = tokens;
+  a.kv_heads = kv_heads;
+  a.heads = heads;
+  a.scale = scale;
+  a.q = q;
+  a.q_ts = q_ts;
+  a.q_hs = q_hs;
+  a.out = out;
+  a.lse = lse;
+  a.err = h->d_err;
+  if (page_size % wp::kKv4Tile) return fail(h, WP_ERR_INVALID, "kv4_attention: page_size must be a multiple of 16");
+  if (int rc = check_seqs(h, "kv4_attention", a, head_dim, dtype)) return rc;
+  if (heads < 1 || heads % kv_heads)
+    return fail(h, WP_ERR_INVALID, "kv4_attention: heads (%d) must be a multiple of kv_heads (%d)", heads, kv_heads);
+  if (num_seqs == 0 || tokens == 0) return WP_OK;
+  if (num_pages < 1) return fail(h, WP_ERR_INVALID, "kv4_attention: the cache has no pages");
+  if (!rows_ok(q, q_ts, q_hs))
+    return fail(h, WP_ERR_INVALID, "kv4_attention: q needs 16-byte aligned rows (strides in multiples of 8 elements)");
+  if (!out || !al16(out)) return fail(h, WP_ERR_INVALID, "kv4_attention: out must be 16-byte aligned");
+  max_q = std::max(max_q, 1);
+  DeviceGuard dg(h->device);
+  const int64_t need = wp::kv4_attention_workspace(dtype, head_dim, heads / kv_heads, max_q, h->num_sms);
+  if (!workspace || !al16(workspace) || workspace_bytes < need)
+    return fail(h, WP_ERR_INVALID, "kv4_attention: needs a 16-byte aligned workspace of %lld bytes",
+                static_cast<long long>(need));
+  cudaError_t e = wp::launch_kv4_attention(dtype, head_dim, max_q, a, workspace, h->num_sms,
+                                           static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(h, WP_ERR_CUDA, "kv4_attention launch: %s", cudaGetErrorString(e));
+  h->launches += 2;
+  return WP_OK;
+}
+
+int wp_token_logprobs(wp_handle* h, float* logprob, int32_t* rank, float* entropy, int32_t* top_ids, float* top_logprobs,
+                      const void* logits, int64_t ld, const void* tokens, int32_t token_dtype, int32_t rows,
+                      int32_t vocab, int32_t top, int32_t dtype, void* stream) {
+  if (!h) return fail(nullptr, WP_ERR_INVALID, "token_logprobs: NULL handle");
+  if (!dtype16(dtype) && dtype != WP_DTYPE_F32)
+    return fail(h, WP_ERR_INVALID, "token_logprobs: logits must be fp16, bf16 or fp32");
+  if (token_dtype != WP_DTYPE_I32 && token_dtype != WP_DTYPE_I64)
+    return fail(h, WP_ERR_INVALID, "token_logprobs: tokens must be int32 or int64");
+  if (rows < 0 || vocab < 1 || ld < vocab) return fail(h, WP_ERR_INVALID, "token_logprobs: bad sizes");
+  if (top < 0 || top > wp::kMaxTop || top > vocab)
+    return fail(h, WP_ERR_INVALID, "token_logprobs: top must be 0..%d and at most the vocabulary", wp::kMaxTop);
+  if (rows == 0) return WP_OK;
+  if (!logprob || !logits || !tokens || (top > 0 && (!top_ids || !top_logprobs)))
+    return fail(h, WP_ERR_INVALID, "token_logprobs: NULL pointer");
+  wp::LogprobArgs a{};
+  a.logits = logits;
+  a.ld = ld;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.tokens = tokens;
+  a.tokens64 = token_dtype == WP_DTYPE_I64;
+  a.top = top;
+  a.logprob = logprob;
+  a.rank = rank;
+  a.entropy = entropy;
+  a.top_ids = top_ids;
+  a.top_logprobs = top_logprobs;
+  DeviceGuard dg(h->device);
+  cudaError_t e = wp::launch_token_logprobs(dtype, a, h->num_sms, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(h, WP_ERR_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
+  ++h->launches;
+  return WP_OK;
+}
+
 }  // extern "C"

@@ -227,4 +227,65 @@ cudaError_t launch_seg_bounds(const void* idx, int idx_dtype, int T, DevSeg* seg
 // 16-byte-addressable y.
 cudaError_t launch_prefill(int dtype, int rank, const ApplyArgs& a, const LaunchCfg& lc);
 
+// ---- 4-bit paged key/value cache (wp_kv4.cu) --------------------------------
+
+// Tokens of one tile, the unit of the cache's layout (include/wp_api.h,
+// wp_kv4_append), and tokens of one stage of the attention kernel.
+constexpr int kKv4Tile = 16;
+constexpr int kKv4Chunk = 64;
+__host__ __device__ constexpr int kv4_tile_bytes(int head_dim) { return 16 * head_dim + 128; }
+
+struct Kv4Args {
+  uint8_t* pages;  // [num_pages][kv_heads][page_tiles][tile_bytes]
+  const int* table;  // [num_seqs][table_ld] page numbers
+  const int* lens;  // [num_seqs] tokens of each sequence, the call's own included
+  const int* cu;  // [num_seqs + 1] offsets of each sequence's tokens in the packed rows; null: one token each
+  int64_t table_ld;
+  int num_pages;
+  int page_tiles;
+  int num_seqs;
+  int tokens;  // packed rows
+  int kv_heads;
+  int heads;
+  float scale;
+  const void* q;
+  void* k;  // append: source; read: destination
+  void* v;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // strides of tokens and heads, in elements
+  void* out;  // [tokens][heads][D]
+  float* lse;  // [tokens][heads] or null
+  float* part;  // partial rows of sequences shared by several warps, [2 per warp][rows][D]
+  float2* part_ml;  // their running maximum (log2 units) and sum, [2 per warp][rows]
+  int4* part_desc;  // [warp][2]: the shared segment that starts in this warp's range
+  int* err;
+};
+
+cudaError_t launch_kv4_append(int dtype, int head_dim, const Kv4Args& a, cudaStream_t stream);
+cudaError_t launch_kv4_read(int dtype, int head_dim, const Kv4Args& a, cudaStream_t stream);
+// Bytes of the partial rows, for calls whose sequences bring at most
+// max_q query tokens; 0 when the kernel cannot run here.
+int64_t kv4_attention_workspace(int dtype, int head_dim, int group, int max_q, int num_sms);
+cudaError_t launch_kv4_attention(int dtype, int head_dim, int max_q, Kv4Args a, void* workspace, int num_sms,
+                                 cudaStream_t stream);
+
+// ---- log probabilities of given tokens (wp_logprobs.cu) ------------------------
+
+constexpr int kMaxTop = 32;  // alternatives per row
+struct LogprobArgs {
+  const void* logits;  // [rows][ld]
+  int64_t ld;
+  int rows;
+  int vocab;
+  const void* tokens;  // [rows] int32 or int64
+  int tokens64;
+  int top;
+  float* logprob;
+  int* rank;  // or null
+  float* entropy;  // or null
+  int* top_ids;  // [rows][top]
+  float* top_logprobs;
+};
+// dtype: WP_DTYPE_F16 / BF16 / F32
+cudaError_t launch_token_logprobs(int dtype, const LogprobArgs& a, int num_sms, cudaStream_t stream);
+
 }  // namespace wp

@@ -22,7 +22,7 @@ Differences from the reference, all widening what is handled:
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -41,6 +41,33 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
 
 def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def _index(t: torch.Tensor, what: str, dims: int) -> torch.Tensor:
+    """An index tensor as the kernels take it: int32, CUDA, contiguous."""
+    if not t.is_cuda or t.dtype != torch.int32 or t.dim() != dims:
+        raise RuntimeError(f"{what} must be a {dims}-d int32 CUDA tensor")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _packed_rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    """[tokens, heads, dim] with rows that 16-byte loads can take, copied only
+    when the strides or the address do not allow them."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} must be a CUDA tensor")
+    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+class TokenLogprobs(NamedTuple):
+    """Result of WarpPipeEngine.token_logprobs."""
+
+    logprob: torch.Tensor  # [rows] fp32
+    rank: torch.Tensor  # [rows] int32
+    entropy: torch.Tensor  # [rows] fp32
+    top_ids: torch.Tensor  # [rows, top] int32
+    top_logprobs: torch.Tensor  # [rows, top] fp32
 
 
 class WarpPipeEngine:
@@ -324,6 +351,39 @@ class WarpPipeEngine:
             int(x2d.size(1)), int(wb_t_all.size(-2)), rank, int(x2d.stride(0)), int(base.stride(0)), 0, dt,
             _stream_ptr(x.device)))
         return True
+
+    # -- scoring (no counterpart in the reference) ---------------------------------
+    def token_logprobs(self, logits, tokens, top: int = 0) -> TokenLogprobs:
+        """Log probability, rank (1 + larger logits) and entropy for one given
+        token per row of logits [rows, vocab] (fp16, bf16 or fp32), and the
+        `top` (at most 32) largest alternatives, equal logits by ascending id.
+        tokens [rows] int32 or int64; one outside the vocabulary has log
+        probability -inf."""
+        if not (logits.is_cuda and tokens.is_cuda):
+            raise RuntimeError("token_logprobs: logits/tokens must be CUDA tensors")
+        code = _lib.WP_DTYPE_F32 if logits.dtype == torch.float32 else _dtype_code(logits, "token_logprobs: logits")
+        if tokens.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError("token_logprobs: tokens must be int32 or int64")
+        if logits.dim() != 2 or tokens.dim() != 1 or int(tokens.size(0)) != int(logits.size(0)):
+            raise RuntimeError("token_logprobs: logits must be [rows, vocab] and tokens [rows]")
+        rows, vocab = int(logits.size(0)), int(logits.size(1))
+        top = int(top)
+        if top < 0 or top > 32 or top > vocab:
+            raise RuntimeError(f"token_logprobs: top must be 0..32 and at most the vocabulary ({vocab}), got {top}")
+        if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
+            logits = logits.contiguous()
+        tokens = tokens.contiguous()
+        dev = logits.device
+        f = torch.empty(rows * (2 + top), dtype=torch.float32, device=dev)
+        i = torch.empty(rows * (1 + top), dtype=torch.int32, device=dev)
+        res = TokenLogprobs(f[:rows], i[:rows], f[rows:2 * rows], i[rows:].view(rows, top), f[2 * rows:].view(rows, top))
+        fp, ip = f.data_ptr(), i.data_ptr()
+        self._check(self._lib.wp_token_logprobs(
+            self._h, fp, ip, fp + 4 * rows, ip + 4 * rows, fp + 8 * rows, logits.data_ptr(),
+            max(int(logits.stride(0)), vocab), tokens.data_ptr(),
+            _lib.WP_DTYPE_I64 if tokens.dtype == torch.int64 else _lib.WP_DTYPE_I32, rows, vocab, top, code,
+            _stream_ptr(dev)))
+        return res
 
     # -- staging slots (engine.py:44-54) -----------------------------------------
     def prefetch_adapter(self, adapter_id) -> int:

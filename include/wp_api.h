@@ -428,6 +428,71 @@ int wp_add_lora_row_parallel(wp_handle* h, void* y, const void* x, const void* w
                              int32_t d_shard, int32_t out_features, int32_t rank, int64_t x_ld, int64_t y_ld,
                              int32_t y_offset, int32_t dtype, void* stream);
 
+/* ---- operators around the LoRA projections (no counterpart in the reference) ---- */
+
+/* A paged key/value cache held in 4 bits. Per token and kv head, K and V each
+ * have a (scale, zero) pair in the cache's 16-bit type: zero = min, scale =
+ * round16((max - min) * (1/15)), code = rint((x - zero) / scale) clamped to
+ * 0..15 (0 where scale is 0), in fp32; a code stands for zero + scale * code.
+ *
+ * pages: DEVICE [num_pages][kv_heads][page_size / 16][tile bytes], 16-byte
+ * aligned, page_size a multiple of 16, head_dim D = 64 or 128. A tile of 16
+ * tokens is wp_kv4_tile_bytes(D) = 16 D + 128 bytes:
+ *   K codes  [16 tokens][D / 2]: byte b holds dimension 2b (low half), 2b + 1
+ *   V codes  [D / 64][8 g][4 c][4 m][4 j]: token 2c + (j >> 1) + 8 (j & 1),
+ *            dimension 64 h + 16 m + g in the low half, 8 further in the high
+ *   K (scale, zero) [16 tokens][2], V (scale, zero) [16 tokens][2]
+ *
+ * Sequence b's token at position p is in page table[b * table_ld + p /
+ * page_size]. lens[b] is its length with this call's tokens included; its
+ * rows in the packed tensors are cu[b] .. cu[b + 1] (cu may be NULL: one token
+ * each), the last ones of the sequence. All three are DEVICE int32 arrays and
+ * are read by the kernels only (graph-capturable). A page number, length or
+ * offset outside its array raises the handle's device error word
+ * (wp_device_error) and is not followed. */
+int64_t wp_kv4_tile_bytes(int32_t head_dim);
+
+/* Stores the packed k and v rows [tokens, kv_heads, D] (strides of tokens and
+ * heads in elements, multiples of 8) at the sequences' last positions. */
+int wp_kv4_append(wp_handle* h, void* pages, int32_t num_pages, int32_t page_size, const void* k, int64_t k_ts,
+                  int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, const int32_t* table, int64_t table_ld,
+                  const int32_t* lens, const int32_t* cu, int32_t num_seqs, int32_t tokens, int32_t kv_heads,
+                  int32_t head_dim, int32_t dtype, void* stream);
+
+/* The reverse: the values that the sequences' last positions stand for, as
+ * contiguous [tokens, kv_heads, D] k and v. */
+int wp_kv4_read(wp_handle* h, void* k, void* v, const void* pages, int32_t num_pages, int32_t page_size,
+                const int32_t* table, int64_t table_ld, const int32_t* lens, const int32_t* cu, int32_t num_seqs,
+                int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t dtype, void* stream);
+
+/* Attention of each sequence's last tokens over the cache, causal: query i of
+ * n sees the positions < lens[b] - (n - 1 - i). q [tokens, heads, D] (query
+ * head j reads kv head j / (heads / kv_heads)), out contiguous [tokens, heads,
+ * D], lse (may be NULL) [tokens, heads] fp32 log of the softmax denominator.
+ * A row that sees nothing is 0 with lse -inf; what a row must not see does not
+ * reach it, NaN and infinities included. max_q: the most query tokens of one
+ * sequence (chooses the kernel; any value is correct). workspace: DEVICE
+ * scratch of at least wp_kv4_attention_workspace bytes, 16-byte aligned,
+ * free for the caller again once the stream has passed the call. */
+int64_t wp_kv4_attention_workspace(wp_handle* h, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t max_q,
+                                   int32_t dtype);
+int wp_kv4_attention(wp_handle* h, void* out, float* lse, const void* q, int64_t q_ts, int64_t q_hs, const void* pages,
+                     int32_t num_pages, int32_t page_size, const int32_t* table, int64_t table_ld, const int32_t* lens,
+                     const int32_t* cu, int32_t num_seqs, int32_t max_q, int32_t tokens, int32_t heads,
+                     int32_t kv_heads, int32_t head_dim, float scale, int32_t dtype, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* Per row of logits [rows, vocab] (row stride ld; fp16, bf16 or fp32): the
+ * log probability of tokens[row], its rank (1 + the number of larger logits),
+ * the entropy of the row's distribution (nats), and the `top` (0..32) largest
+ * logits as ids, equal ones by ascending id, with their log probabilities.
+ * rank and entropy may be NULL. A token outside the vocabulary has log
+ * probability -inf. A row of only -inf: log probabilities -inf, entropy 0; a
+ * row with NaN or +inf: NaN. */
+int wp_token_logprobs(wp_handle* h, float* logprob, int32_t* rank, float* entropy, int32_t* top_ids, float* top_logprobs,
+                      const void* logits, int64_t ld, const void* tokens, int32_t token_dtype, int32_t rows,
+                      int32_t vocab, int32_t top, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
