@@ -148,6 +148,8 @@ SIGNATURES = {
     "wp_build_seg_bounds_ex": (_int, [_vp, _vp, _i32, _i32, _i32, _vp]),
     "wp_write_bridge": (_int, [_vp, ctypes.POINTER(WpBridge)]),
     "wp_read_bridge": (_int, [_vp, ctypes.POINTER(WpBridge)]),
+    "wp_prompt_attention": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32,
+                                   _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp]),
     "wp_kv4_tile_bytes": (_i64, [_i32]),
     "wp_kv4_append": (_int, [_vp, _vp, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i32, _i32,
                              _i32, _i32, _i32, _vp]),

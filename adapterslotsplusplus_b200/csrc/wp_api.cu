@@ -2189,4 +2189,51 @@ int wp_token_logprobs(wp_handle* h, float* logprob, int32_t* rank, float* entrop
   return WP_OK;
 }
 
+int wp_prompt_attention(wp_handle* h, void* out, float* lse, const void* q, int64_t q_ts, int64_t q_hs, const void* k,
+                        int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, const int32_t* cu_q,
+                        const int32_t* cu_k, int32_t num_seqs, int32_t max_q, int32_t q_tokens, int32_t k_tokens,
+                        int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, int32_t dtype, void* stream) {
+  if (!h) return fail(nullptr, WP_ERR_INVALID, "prompt_attention: NULL handle");
+  if (!dtype16(dtype)) return fail(h, WP_ERR_INVALID, "prompt_attention: dtype must be fp16 or bf16");
+  if (head_dim < 8 || head_dim > 128 || head_dim % 8)
+    return fail(h, WP_ERR_INVALID, "prompt_attention: head_dim must be a multiple of 8 up to 128, got %d", head_dim);
+  if (kv_heads < 1 || kv_heads > 65535 || heads < 1 || heads % kv_heads)
+    return fail(h, WP_ERR_INVALID, "prompt_attention: heads (%d) must be a multiple of kv_heads (%d)", heads, kv_heads);
+  if (num_seqs < 0 || q_tokens < 0 || k_tokens < 0) return fail(h, WP_ERR_INVALID, "prompt_attention: bad sizes");
+  if (num_seqs == 0 || q_tokens == 0) return WP_OK;
+  if (!cu_q || !cu_k) return fail(h, WP_ERR_INVALID, "prompt_attention: NULL offsets");
+  if (!rows_ok(q, q_ts, q_hs) || (k_tokens > 0 && (!rows_ok(k, k_ts, k_hs) || !rows_ok(v, v_ts, v_hs))))
+    return fail(h, WP_ERR_INVALID,
+                "prompt_attention: q, k and v need 16-byte aligned rows (strides in multiples of 8 elements)");
+  if (!out || !al16(out)) return fail(h, WP_ERR_INVALID, "prompt_attention: out must be 16-byte aligned");
+  wp::PromptArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.lse = lse;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.q_ts = q_ts;
+  a.q_hs = q_hs;
+  a.k_ts = k_ts;
+  a.k_hs = k_hs;
+  a.v_ts = v_ts;
+  a.v_hs = v_hs;
+  a.num_seqs = num_seqs;
+  a.q_tokens = q_tokens;
+  a.k_tokens = k_tokens;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = head_dim;
+  a.max_q = std::min(std::max(max_q, 1), q_tokens);
+  a.scale = scale;
+  a.err = h->d_err;
+  DeviceGuard dg(h->device);
+  cudaError_t e = wp::launch_prompt_attention(dtype, a, h->num_sms, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(h, WP_ERR_CUDA, "prompt_attention launch: %s", cudaGetErrorString(e));
+  ++h->launches;
+  return WP_OK;
+}
+
 }  // extern "C"

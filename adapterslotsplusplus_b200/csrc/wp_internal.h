@@ -288,4 +288,27 @@ struct LogprobArgs {
 // dtype: WP_DTYPE_F16 / BF16 / F32
 cudaError_t launch_token_logprobs(int dtype, const LogprobArgs& a, int num_sms, cudaStream_t stream);
 
+// ---- attention over packed prompts (wp_attention.cu) ---------------------------
+
+struct PromptArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;  // [q_tokens][heads][dim]
+  float* lse;  // [q_tokens][heads] or null
+  const int* cu_q;  // [num_seqs + 1]
+  const int* cu_k;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // strides of tokens and heads, in elements
+  int num_seqs;
+  int q_tokens;
+  int k_tokens;
+  int heads;
+  int kv_heads;
+  int dim;
+  int max_q;
+  float scale;
+  int* err;
+};
+cudaError_t launch_prompt_attention(int dtype, const PromptArgs& a, int num_sms, cudaStream_t stream);
+
 }  // namespace wp

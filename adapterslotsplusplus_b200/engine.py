@@ -352,6 +352,43 @@ class WarpPipeEngine:
             _stream_ptr(x.device)))
         return True
 
+    # -- attention over prompts (no counterpart in the reference) -------------------
+    def prompt_attention(self, q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: Optional[float] = None,
+                         return_lse: bool = False):
+        """Causal attention over packed prompts of different lengths: q
+        [tokens, heads, dim], k and v [key tokens, kv_heads, dim], heads a
+        multiple of kv_heads, dim a multiple of 8 up to 128, fp16 or bf16.
+        cu_q [sequences + 1] (int32) are the offsets of each sequence's rows;
+        cu_k those of its keys where they differ (a chunk behind its context:
+        query i of nq sees the keys j <= i + nk - nq). scale defaults to
+        dim ** -0.5; max_q, the most query tokens of one sequence, chooses the
+        kernel only. Returns out like q (contiguous), and the softmax's log
+        denominators [tokens, heads] in fp32 with return_lse. A row that sees
+        no key is 0 (lse -inf)."""
+        if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape != v.shape:
+            raise RuntimeError("prompt_attention: q must be [tokens, heads, dim], k and v [key tokens, kv_heads, dim]")
+        dt = _dtype_code(q, "prompt_attention: q/k/v")
+        if k.dtype != q.dtype or v.dtype != q.dtype:
+            raise RuntimeError("prompt_attention: q, k and v must share one dtype")
+        tokens, heads, dim = q.shape
+        keys, kv_heads, k_dim = k.shape
+        if k_dim != dim or kv_heads == 0 or heads == 0 or heads % kv_heads:
+            raise RuntimeError(f"prompt_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not go together")
+        q, k, v = (_packed_rows(t, "prompt_attention: q/k/v") for t in (q, k, v))
+        cu_q = _index(cu_q, "prompt_attention: cu_q", 1)
+        cu_k = cu_q if cu_k is None else _index(cu_k, "prompt_attention: cu_k", 1)
+        n = int(cu_q.numel()) - 1
+        if n < 0 or int(cu_k.numel()) != n + 1:
+            raise RuntimeError("prompt_attention: cu_q and cu_k must have one entry more than there are sequences")
+        out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=q.device)
+        lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
+        self._check(self._lib.wp_prompt_attention(
+            self._h, out.data_ptr(), None if lse is None else lse.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cu_q.data_ptr(),
+            cu_k.data_ptr(), n, tokens if max_q is None else int(max_q), tokens, keys, heads, kv_heads, dim,
+            dim ** -0.5 if scale is None else float(scale), dt, _stream_ptr(q.device)))
+        return (out, lse) if return_lse else out
+
     # -- scoring (no counterpart in the reference) ---------------------------------
     def token_logprobs(self, logits, tokens, top: int = 0) -> TokenLogprobs:
         """Log probability, rank (1 + larger logits) and entropy for one given

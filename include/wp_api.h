@@ -430,6 +430,22 @@ int wp_add_lora_row_parallel(wp_handle* h, void* y, const void* x, const void* w
 
 /* ---- operators around the LoRA projections (no counterpart in the reference) ---- */
 
+/* Causal attention over packed prompts with grouped heads. q [q_tokens, heads,
+ * D], k and v [k_tokens, kv_heads, D] (strides of tokens and heads in
+ * elements, multiples of 8; 16-byte aligned; D a multiple of 8 up to 128),
+ * out contiguous [q_tokens, heads, D], lse (may be NULL) [q_tokens, heads]
+ * fp32. Sequence b has query rows cu_q[b] .. cu_q[b + 1] and key rows cu_k[b]
+ * .. cu_k[b + 1] (DEVICE int32, num_seqs + 1 each, the same array for prompts
+ * without context); query i of nq sees the keys j <= i + nk - nq. A row that
+ * sees no key is 0 with lse -inf; what a row must not see does not reach it.
+ * max_q: the most query tokens of one sequence (chooses the kernel; any value
+ * is correct). Offsets outside the packed tensors raise the device error word
+ * and are cut. */
+int wp_prompt_attention(wp_handle* h, void* out, float* lse, const void* q, int64_t q_ts, int64_t q_hs, const void* k,
+                        int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, const int32_t* cu_q,
+                        const int32_t* cu_k, int32_t num_seqs, int32_t max_q, int32_t q_tokens, int32_t k_tokens,
+                        int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, int32_t dtype, void* stream);
+
 /* A paged key/value cache held in 4 bits. Per token and kv head, K and V each
  * have a (scale, zero) pair in the cache's 16-bit type: zero = min, scale =
  * round16((max - min) * (1/15)), code = rint((x - zero) / scale) clamped to
