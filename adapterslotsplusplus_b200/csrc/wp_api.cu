@@ -225,6 +225,13 @@ bool encode_map(CUtensorMap* m, int dtype, int rank, const void* base, const uin
   return r == CUDA_SUCCESS;
 }
 
+}  // namespace
+bool wp::encode_tiled_map(CUtensorMap* m, int dtype, int rank, const void* base, const uint64_t* dims,
+                          const uint64_t* strides, const uint32_t* box) {
+  return encode_map(m, dtype, rank, base, dims, strides, box);
+}
+namespace {
+
 // A stack [L, r, d] (row stride d, adapter stride `stride0` elements): box 64 x r x 1.
 // d (A, x) or o (y) allows the sliced view [cols / 64][64] of a row.
 bool sliced(int cols) { return cols % wp::kBoxCols == 0; }

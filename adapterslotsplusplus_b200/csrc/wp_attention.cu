@@ -50,7 +50,7 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptArgs& a, int b) {
 // that key's V, which is NaN where V is not finite; rows whose result is not
 // finite come here, so only a row's own keys decide what it is.
 template <typename T>
-__device__ __noinline__ void prompt_row(const PromptArgs& a, const PromptSeq& s, int token, int head) {
+__device__ __forceinline__ void prompt_row(const PromptArgs& a, const PromptSeq& s, int token, int head) {
   const int lane = threadIdx.x & 31, d0 = lane * 4, kvh = head / (a.heads / a.kv_heads);
   const bool on = d0 < a.dim;
   auto load = [&](const T* p, float (&x)[4]) {
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(NW * 32) prompt_small_kernel(const __grid_cons
   using C = SmallCfg<T, D, NW>;
   using E = Elem<T>;
   constexpr int BN = C::BN, LD = C::LD, KS = D / 16;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.y, group = a.heads / a.kv_heads;
   const uint32_t ring = smem_u32(smem), qs = ring + 4 * C::TILE + warp * 16 * LD;
@@ -288,9 +288,446 @@ cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+// ---- many query rows: tcgen05 -----------------------------------------------------
+//
+// A work item is (sequence, kv head, pair of 128-row tiles of packed query
+// rows). Per 128 keys: S_i = Q_i K^T and O_i += P_i V for both tiles i, four
+// tcgen05.mma groups of 128 x 128 x D. S and O live in TMEM (2 x 128 + 2 x D
+// columns of 512); the weights P go back into S's own columns as 16-bit pairs
+// and are the second product's A operand from there, so they never touch
+// shared memory.
+//
+// Warps (384 threads): 0-3 softmax of tile 0, 4-7 of tile 1 (one thread per
+// row: no exchange between lanes), 8 TMA producer, 9 MMA issuer; 10 and 11 only
+// give their registers to the softmax warps, which hold a row's 128 scores
+// (256 x 216 + 128 x 72 = the launch's 384 x 168). The issuer
+// alternates the tiles: while one tile's softmax runs, the other's P V and
+// next Q K^T keep the tensor core busy. Products of one CTA run in order, so
+// S_i(j + 1) may follow P_i(j) V into the same columns, and the arrival of
+// S_i(j) tells that O_i holds all blocks before j.
+//
+// The running maximum is only raised when a row's grows by more than 8 (in
+// log2 units): weights then reach 2^8 at most, which costs fp16 and bf16
+// nothing, and O is rescaled in a few blocks at the start instead of in most.
+//
+// Persistent: CTA c takes items c, 2 G - 1 - c, 2 G + c, ... in the order
+// (sequence, pairs from the last one, kv head), so long items come first
+// within a sequence and every CTA gets its share of them.
+
+constexpr int kPaWarps = 12;
+constexpr int kPaThreads = kPaWarps * 32;
+constexpr int kPaProd = 8;
+constexpr int kPaMma = 9;
+constexpr int kPaRows = 128;  // rows of a tile
+constexpr int kPaKeys = 128;  // keys of a block
+constexpr float kPaLazy = 8.f;
+
+template <int DP>
+struct PaCfg {
+  static constexpr int SL = DP / 64;  // 64-column slices of a row
+  static constexpr int SLICE = 128 * 128;  // bytes of one slice of 128 rows
+  static constexpr int TILE = SL * SLICE;
+  static constexpr int S = DP == 128 ? 5 : 8;  // ring stages; K and V tiles alternate
+  static constexpr int HEAD = 2048;  // barriers, prefix sums
+  static constexpr int SMEM = HEAD + 1024 + (2 + S) * TILE;
+  static constexpr uint32_t COL_O = 256;
+  static_assert(SMEM <= 232448, "shared memory budget");
+};
+
+struct PaMaps {
+  CUtensorMap q;  // [tokens][heads][dim], box 64 columns x group x tokens of a tile
+  CUtensorMap k, v;  // [tokens][kv heads][dim], box 64 columns x 1 x 128
+};
+
+struct PaItem {
+  PromptSeq s;
+  int kvh;
+  int t0;  // first token of the pair
+  int n[2];  // key blocks of each tile (0: no tokens, or none that sees a key)
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPaThreads, 1)
+    prompt_tile_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PaMaps maps) {
+  using C = PaCfg<DP>;
+  using E = Elem<T>;
+  constexpr int S = C::S;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem);  // [S]
+  uint64_t* kv_empty = kv_full + 8;  // [S]
+  uint64_t* q_full = kv_full + 16;  // [2]
+  uint64_t* q_empty = kv_full + 18;
+  uint64_t* s_full = kv_full + 20;
+  uint64_t* p_full = kv_full + 22;
+  uint64_t* o_full = kv_full + 24;
+  uint64_t* o_free = kv_full + 26;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(kv_full + 28);
+  volatile int* s_bad = reinterpret_cast<volatile int*>(kv_full + 29);
+  int* s_warp = reinterpret_cast<int*>(kv_full + 30);  // [kPaWarps]
+  int* s_sum = reinterpret_cast<int*>(smem + 512);  // items before thread i's slice of sequences
+  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + C::HEAD + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = tiles + 2 * C::TILE;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = a.heads / a.kv_heads;
+  const int tpt = kPaRows / group;  // tokens of a tile
+
+  // ---- items of each thread's slice of sequences, and their prefix sums
+  const int slice = (a.num_seqs + kPaThreads - 1) / kPaThreads;
+  auto pairs_of = [&](int nq) { return (nq + 2 * tpt - 1) / (2 * tpt); };
+  int mine = 0;
+  for (int b = tid * slice; b < min((tid + 1) * slice, a.num_seqs); ++b) mine += pairs_of(prompt_seq(a, b).nq) * a.kv_heads;
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(~0u, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_free[i], 4);
+    }
+    *s_bad = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) tmem_alloc(s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *s_tmem;
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kPaWarps; ++w) {
+    if (w < warp) before += s_warp[w];
+    total += s_warp[w];
+  }
+  s_sum[tid] = before + incl - mine;
+  __syncthreads();
+
+  // The warp's n-th item; false past the last one.
+  auto item = [&](int n, PaItem& it) {
+    const int G = gridDim.x, x = n * G + (n & 1 ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
+    if (n * G >= total) return false;
+    if (x >= total) {  // the last round's tail: nothing for this CTA
+      it.n[0] = it.n[1] = -1;
+      return true;
+    }
+    int sl = 0;
+    for (int i = lane; i < kPaThreads; i += 32)
+      if (s_sum[i] <= x) sl = i;
+    sl = __reduce_max_sync(~0u, sl);
+    int b = sl * slice, y = x - s_sum[sl], pairs;
+    while (true) {
+      it.s = prompt_seq(a, b);
+      pairs = pairs_of(it.s.nq);
+      if (y < pairs * a.kv_heads) break;
+      y -= pairs * a.kv_heads;
+      ++b;
+    }
+    it.kvh = y % a.kv_heads;
+    it.t0 = (pairs - 1 - y / a.kv_heads) * 2 * tpt;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int first = it.t0 + i * tpt, last = min(first + tpt, it.s.nq) - 1;
+      const int end = first < it.s.nq ? min(max(last + it.s.nk - it.s.nq + 1, 0), it.s.nk) : 0;
+      it.n[i] = (end + kPaKeys - 1) / kPaKeys;
+    }
+    return true;
+  };
+
+  PaItem it;
+  if (warp >= kPaProd) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == kPaProd) {
+      // ============================ TMA producer ==============================
+      if (lane == 0) {
+        prefetch_tmap(&maps.q);
+        prefetch_tmap(&maps.k);
+        prefetch_tmap(&maps.v);
+      }
+      const uint32_t q_bytes = static_cast<uint32_t>(C::SL * group * tpt * 128);
+      int u = 0, qn[2] = {0, 0};
+      for (int n = 0; item(n, it); ++n) {
+        const int blocks = max(it.n[0], it.n[1]);
+        if (lane == 0 && !*s_bad) {
+          for (int i = 0; i < 2; ++i) {
+            if (it.n[i] <= 0) continue;
+            if (qn[i] > 0 && !mbar_wait_bounded(&q_empty[i], (qn[i] - 1) & 1, a.err)) *s_bad = 1;
+            ++qn[i];
+            mbar_arrive_expect_tx(&q_full[i], q_bytes);
+            for (int sl = 0; sl < C::SL; ++sl)
+              tma_load_3d(tiles + i * C::TILE + sl * C::SLICE, &maps.q, sl * 64, it.kvh * group, it.s.q0 + it.t0 + i * tpt,
+                          &q_full[i]);
+          }
+          for (int j = 0; j < 2 * blocks && !*s_bad; ++j, ++u) {
+            const int st = u % S;
+            if (u >= S && !mbar_wait_bounded(&kv_empty[st], ((u / S) - 1) & 1, a.err)) {
+              *s_bad = 1;
+              break;
+            }
+            mbar_arrive_expect_tx(&kv_full[st], C::TILE);
+            for (int sl = 0; sl < C::SL; ++sl)
+              tma_load_3d(ring + st * C::TILE + sl * C::SLICE, j & 1 ? &maps.v : &maps.k, sl * 64, it.kvh,
+                          it.s.k0 + (j >> 1) * kPaKeys, &kv_full[st]);
+          }
+        }
+        __syncwarp();
+      }
+      if (lane == 0 && *s_bad)  // a wait ran out: let the copies in flight land before the CTA leaves
+        for (int i = max(u - S, 0); i < u; ++i) mbar_wait_bounded(&kv_full[i % S], (i / S) & 1, a.err);
+    } else if (warp == kPaMma) {
+      // ============================ MMA issuer ================================
+      constexpr uint32_t kAb = E::is_bf16 ? 1u : 0u;
+      const uint32_t id_s = umma_idesc(kAb, kPaRows, kPaKeys);
+      const uint32_t id_o = umma_idesc(kAb, kPaRows, DP) | kUmmaBMajorN;
+      int u = 0, qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};
+      auto wait = [&](uint64_t* bar, int parity) {
+        if (!*s_bad && !mbar_wait_bounded(bar, parity, a.err)) *s_bad = 1;
+      };
+      auto scores = [&](int i, int st) {
+        const uint32_t qa = smem_u32(tiles + i * C::TILE), ka = smem_u32(ring + st * C::TILE);
+  #pragma unroll
+        for (int sl = 0; sl < C::SL; ++sl) {
+          const uint64_t dq = umma_desc(qa + sl * C::SLICE, 1024, 2), dk = umma_desc(ka + sl * C::SLICE, 1024, 2);
+  #pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_f16(tbase + i * kPaKeys, dq + 2 * ks, dk + 2 * ks, id_s, sl > 0 || ks > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[i]);
+      };
+      for (int n = 0; item(n, it); ++n) {
+        const int blocks = max(it.n[0], it.n[1]);
+        if (lane == 0 && blocks > 0) {
+          wait(&kv_full[u % S], (u / S) & 1);  // K(0)
+          tc_fence_after();
+          for (int i = 0; i < 2; ++i)
+            if (it.n[i] > 0 && !*s_bad) {
+              wait(&q_full[i], qn[i]++ & 1);
+              if (!*s_bad) scores(i, u % S);
+              if (it.n[i] == 1) umma_commit(&q_empty[i]);
+            }
+          umma_commit(&kv_empty[u % S]);
+          for (int j = 0; j < blocks && !*s_bad; ++j) {
+            const int sv = (u + 1) % S, sk = (u + 2) % S;
+            wait(&kv_full[sv], ((u + 1) / S) & 1);  // V(j)
+            if (j + 1 < blocks) wait(&kv_full[sk], ((u + 2) / S) & 1);  // K(j + 1)
+            for (int i = 0; i < 2; ++i) {
+              if (j >= it.n[i] || *s_bad) continue;
+              if (j == 0 && on[i]++ > 0) wait(&o_free[i], on[i] & 1);  // the tile's previous output was read
+              wait(&p_full[i], pn[i]++ & 1);
+              if (*s_bad) continue;
+              tc_fence_after();
+              const uint32_t va = smem_u32(ring + sv * C::TILE);
+  #pragma unroll
+              for (int ks = 0; ks < kPaKeys / 16; ++ks)
+                umma_f16_ts(tbase + C::COL_O + i * DP, tbase + i * kPaKeys + ks * 8,
+                            umma_desc_mn(va + ks * 2048, C::SLICE, 1024), id_o, j > 0 || ks > 0 ? 1u : 0u);
+              if (j + 1 < it.n[i]) {
+                scores(i, sk);
+                if (j + 2 == it.n[i]) umma_commit(&q_empty[i]);
+              } else {
+                umma_commit(&o_full[i]);
+              }
+            }
+            umma_commit(&kv_empty[sv]);
+            if (j + 1 < blocks) umma_commit(&kv_empty[sk]);
+            u += 2;
+          }
+        }
+        __syncwarp();
+      }
+      if (lane == 0 && *s_bad) {  // let the products in flight end before TMEM is freed
+        umma_commit(&o_full[0]);
+        mbar_wait_bounded(&o_full[0], 0, a.err, 1000000ull);
+      }
+    }
+  } else {
+    // ============================ softmax, one thread per row ================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int i = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t ts = tbase + i * kPaKeys + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t to = tbase + C::COL_O + i * DP + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float sc = a.scale * kLog2e;
+    int sn = 0, on = 0;
+    for (int n = 0; item(n, it) && !*s_bad; ++n) {
+      const int first = it.t0 + i * tpt;
+      const int blocks = i ? it.n[1] : it.n[0];
+      if (blocks < 0 || first >= it.s.nq) continue;
+      const int token = first + row / group, head = it.kvh * group + row % group;
+      const bool live = row < tpt * group && token < it.s.nq;
+      const int shift = it.s.nk - it.s.nq + 1;
+      const int lim = min(token + shift, it.s.nk);  // keys this row sees
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < blocks; ++j) {
+        if (!mbar_wait_bounded(&s_full[i], sn++ & 1, a.err)) {
+          *s_bad = 1;
+          break;
+        }
+        tc_fence_after();
+        uint32_t x[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32_nowait(ts + q * 32, x[q]);
+        tmem_wait_ld();
+        if ((j + 1) * kPaKeys > first + shift) {  // some row of the tile sees less than the whole block
+          const int left = lim - j * kPaKeys;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (q * 32 + e >= left) x[q][e] = 0xff800000u;
+        }
+        float t[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          t[q] = __uint_as_float(x[q][0]);
+#pragma unroll
+          for (int e = 1; e < 32; ++e) t[q] = fmaxf(t[q], __uint_as_float(x[q][e]));
+        }
+        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        if (__any_sync(~0u, (top - m) * sc > kPaLazy || (m == -INFINITY && top > m))) {
+          const float mn = fmaxf(m, top);
+          const float f = m == -INFINITY ? 0.f : ex2((m - mn) * sc);
+          m = mn;
+          l *= f;
+          if (j > 0) {
+#pragma unroll
+            for (int q = 0; q < DP / 32; ++q) {
+              uint32_t o[32];
+              tmem_ld32_nowait(to + q * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32_nowait(to + q * 32, o);
+            }
+          }
+        }
+        const float off = m == -INFINITY ? 0.f : -m * sc;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t p[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float p0 = ex2(fmaf(__uint_as_float(x[2 * h + e / 16][(2 * e) % 32]), sc, off));
+            const float p1 = ex2(fmaf(__uint_as_float(x[2 * h + e / 16][(2 * e) % 32 + 1]), sc, off));
+            sum[e & 1] += p0;
+            sum[2 + (e & 1)] += p1;
+            p[e] = E::pack2(p0, p1);
+          }
+          tmem_st32_nowait(ts + h * 32, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[i]);
+      }
+      // ---- the tile's output
+      const int64_t at = static_cast<int64_t>(it.s.q0 + token) * a.heads + head;
+      T* op = static_cast<T*>(a.out) + at * a.dim;
+      bool odd = false;
+      if (blocks > 0) {
+        if (*s_bad || !mbar_wait_bounded(&o_full[i], on++ & 1, a.err)) {
+          *s_bad = 1;
+          break;
+        }
+        tc_fence_after();
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int q = 0; q < DP / 32; ++q) {
+          uint32_t o[32];
+          tmem_ld32_nowait(to + q * 32, o);
+          tmem_wait_ld();
+          if (q == DP / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[i]);
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              y[e] = __uint_as_float(o[8 * w + e]) * inv;
+              odd |= !(fabsf(y[e]) <= 3e38f);
+            }
+            if (live && q * 32 + w * 8 < a.dim)
+              *reinterpret_cast<uint4*>(op + q * 32 + w * 8) =
+                  make_uint4(E::pack2(y[0], y[1]), E::pack2(y[2], y[3]), E::pack2(y[4], y[5]), E::pack2(y[6], y[7]));
+          }
+        }
+      } else if (live) {  // no row of the tile sees a key
+        for (int d = 0; d < a.dim; d += 8) *reinterpret_cast<uint4*>(op + d) = make_uint4(0, 0, 0, 0);
+      }
+      if (a.lse && live) a.lse[at] = l == 0.f ? -INFINITY : (m * sc + __log2f(l)) * kLn2;
+      for (unsigned todo = __ballot_sync(~0u, odd && live); todo; todo &= todo - 1) {
+        const int r = (warp & 3) * 32 + __ffs(todo) - 1;
+        prompt_row<T>(a, it.s, first + r / group, it.kvh * group + r % group);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 512);
+  }
+}
+
+// A [tokens][heads][dim] tensor in boxes of 64 columns x box_heads x box_tokens.
+bool prompt_map(CUtensorMap* m, int dtype, const void* base, int dim, int heads, int tokens, int64_t ts, int64_t hs,
+                int box_heads, int box_tokens) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(hs) * 2, static_cast<uint64_t>(ts) * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(box_heads), static_cast<uint32_t>(box_tokens)};
+  return encode_tiled_map(m, dtype, 3, base, dims, strides, box);
+}
+
+template <typename T, int DP>
+cudaError_t launch_tiles(int dtype, const PromptArgs& a, int num_sms, cudaStream_t stream) {
+  using C = PaCfg<DP>;
+  static std::atomic<bool> ready{false};
+  if (!ready.load()) {
+    cudaError_t e = cudaFuncSetAttribute(prompt_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    ready.store(true);
+  }
+  const int group = a.heads / a.kv_heads, tpt = kPaRows / group;
+  PaMaps maps;
+  if (!prompt_map(&maps.q, dtype, a.q, a.dim, a.heads, a.q_tokens, a.q_ts, a.q_hs, group, tpt) ||
+      !prompt_map(&maps.k, dtype, a.k, a.dim, a.kv_heads, a.k_tokens, a.k_ts, a.k_hs, 1, kPaKeys) ||
+      !prompt_map(&maps.v, dtype, a.v, a.dim, a.kv_heads, a.k_tokens, a.v_ts, a.v_hs, 1, kPaKeys))
+    return cudaErrorInvalidValue;
+  const int64_t most = (static_cast<int64_t>(a.q_tokens) / (2 * tpt) + a.num_seqs) * a.kv_heads;
+  prompt_tile_kernel<T, DP><<<static_cast<unsigned>(std::min<int64_t>(num_sms, most)), kPaThreads, C::SMEM, stream>>>(a, maps);
+  return cudaGetLastError();
+}
+
+// The tiled kernel takes sequences that fill a good part of a tile, with
+// strides a tensor map can express; its maxima are of unscaled scores, so the
+// scale has to be positive.
+bool use_tiles(const PromptArgs& a) {
+  const int group = a.heads / a.kv_heads;
+  const int64_t rows = static_cast<int64_t>(a.max_q) * group;
+  const int64_t most = int64_t{1} << 38;
+  auto ok = [&](int64_t s) { return s > 0 && s < most; };
+  return rows >= 64 && group <= kPaRows && a.k_tokens > 0 && a.scale > 0.f && a.scale < 1e30f && ok(a.q_ts) && ok(a.q_hs) &&
+         ok(a.k_ts) && ok(a.k_hs) && ok(a.v_ts) && ok(a.v_hs);
+}
+
 template <typename T>
-cudaError_t launch_prompt(const PromptArgs& a, int num_sms, cudaStream_t stream) {
-  (void)num_sms;
+cudaError_t launch_prompt(int dtype, const PromptArgs& a, int num_sms, cudaStream_t stream) {
+  if (use_tiles(a))
+    return a.dim <= 64 ? launch_tiles<T, 64>(dtype, a, num_sms, stream) : launch_tiles<T, 128>(dtype, a, num_sms, stream);
   const int64_t rows = static_cast<int64_t>(a.max_q) * (a.heads / a.kv_heads);
   if (a.dim <= 64)
     return rows <= 16 ? launch_small<T, 64, 1>(a, stream) : launch_small<T, 64, 4>(a, stream);
@@ -300,7 +737,8 @@ cudaError_t launch_prompt(const PromptArgs& a, int num_sms, cudaStream_t stream)
 }  // namespace
 
 cudaError_t launch_prompt_attention(int dtype, const PromptArgs& a, int num_sms, cudaStream_t stream) {
-  return dtype == 1 ? launch_prompt<__nv_bfloat16>(a, num_sms, stream) : launch_prompt<__half>(a, num_sms, stream);
+  return dtype == 1 ? launch_prompt<__nv_bfloat16>(dtype, a, num_sms, stream)
+                    : launch_prompt<__half>(dtype, a, num_sms, stream);
 }
 
 }  // namespace wp

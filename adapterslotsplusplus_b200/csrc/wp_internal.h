@@ -288,6 +288,11 @@ struct LogprobArgs {
 // dtype: WP_DTYPE_F16 / BF16 / F32
 cudaError_t launch_token_logprobs(int dtype, const LogprobArgs& a, int num_sms, cudaStream_t stream);
 
+// Tensor map over 16-bit elements (dtype 1: bf16) with the 128-byte swizzle;
+// strides in bytes for dims 1..rank-1 (wp_api.cu).
+bool encode_tiled_map(CUtensorMap* m, int dtype, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                      const uint32_t* box);
+
 // ---- attention over packed prompts (wp_attention.cu) ---------------------------
 
 struct PromptArgs {
