@@ -61,6 +61,7 @@ __device__ __forceinline__ void prompt_row(const PromptArgs& a, const PromptSeq&
   float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
   load(static_cast<const T*>(a.q) + static_cast<int64_t>(s.q0 + token) * a.q_ts + head * a.q_hs, q);
   const int end = min(token + s.nk - s.nq + 1, s.nk);
+#pragma unroll 1
   for (int j = 0; j < end; ++j) {
     float k[4], v[4];
     load(static_cast<const T*>(a.k) + static_cast<int64_t>(s.k0 + j) * a.k_ts + kvh * a.k_hs, k);
@@ -298,13 +299,17 @@ cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
 // shared memory.
 //
 // Warps (384 threads): 0-3 softmax of tile 0, 4-7 of tile 1 (one thread per
-// row: no exchange between lanes), 8 TMA producer, 9 MMA issuer; 10 and 11 only
-// give their registers to the softmax warps, which hold a row's 128 scores
-// (256 x 216 + 128 x 72 = the launch's 384 x 168). The issuer
-// alternates the tiles: while one tile's softmax runs, the other's P V and
-// next Q K^T keep the tensor core busy. Products of one CTA run in order, so
-// S_i(j + 1) may follow P_i(j) V into the same columns, and the arrival of
-// S_i(j) tells that O_i holds all blocks before j.
+// row: no exchange between lanes), 8 TMA producer, 9 and 10 MMA issuers of tile
+// 0 and 1; 11 only gives its registers to the softmax warps, which hold a row's
+// 128 scores (256 x 216 + 128 x 72 = the launch's 384 x 168). While one tile's
+// softmax runs, the other's P V and next Q K^T keep the tensor core busy. Each
+// tile has its own issuer because the tensor core queues only a few products,
+// so one issuer's waits for both tiles would drain it; the issuers take turns
+// (`turn`), because two tiles whose products interleave end up with their
+// softmaxes at the same time (608 us against 494 us at the size below). The
+// products of one issuer run in order, so S_i(j + 1) may follow P_i(j) V into
+// the same columns, and the arrival of S_i(j) tells that O_i holds all blocks
+// before j. P V starts on the first 64 keys' weights.
 //
 // The running maximum is only raised when a row's grows by more than 8 (in
 // log2 units): weights then reach 2^8 at most, which costs fp16 and bf16
@@ -321,6 +326,12 @@ constexpr int kPaMma = 9;
 constexpr int kPaRows = 128;  // rows of a tile
 constexpr int kPaKeys = 128;  // keys of a block
 constexpr float kPaLazy = 8.f;
+// Of 8 pairs of weights, those that take the FMA pipe instead of the special-
+// function unit. 8192 tokens, 32 query / 8 kv heads of 128, bf16: 493, 498, 450
+// and 481 us for 0, 1, 2 and 3 (1.22 PFLOP/s, 74% of the measured matrix rate;
+// what bounds it is the chain scores -> maximum -> weights -> products of a
+// tile, 3000-3500 cycles per 128 keys against 2100 of the products themselves).
+constexpr int kPaFma = 2;
 
 template <int DP>
 struct PaCfg {
@@ -358,12 +369,13 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   uint64_t* q_full = kv_full + 16;  // [2]
   uint64_t* q_empty = kv_full + 18;
   uint64_t* s_full = kv_full + 20;
-  uint64_t* p_full = kv_full + 22;
-  uint64_t* o_full = kv_full + 24;
-  uint64_t* o_free = kv_full + 26;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(kv_full + 28);
-  volatile int* s_bad = reinterpret_cast<volatile int*>(kv_full + 29);
-  int* s_warp = reinterpret_cast<int*>(kv_full + 30);  // [kPaWarps]
+  uint64_t* p_full = kv_full + 22;  // [2 tiles][2 halves of the keys]
+  uint64_t* turn = kv_full + 26;  // whose products are next
+  uint64_t* o_full = kv_full + 28;
+  uint64_t* o_free = kv_full + 30;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(kv_full + 32);
+  volatile int* s_bad = reinterpret_cast<volatile int*>(kv_full + 33);
+  int* s_warp = reinterpret_cast<int*>(kv_full + 34);  // [kPaWarps]
   int* s_sum = reinterpret_cast<int*>(smem + 512);  // items before thread i's slice of sequences
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + C::HEAD + 1023) & ~uintptr_t(1023));
   uint8_t* ring = tiles + 2 * C::TILE;
@@ -375,6 +387,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   const int slice = (a.num_seqs + kPaThreads - 1) / kPaThreads;
   auto pairs_of = [&](int nq) { return (nq + 2 * tpt - 1) / (2 * tpt); };
   int mine = 0;
+#pragma unroll 1
   for (int b = tid * slice; b < min((tid + 1) * slice, a.num_seqs); ++b) mine += pairs_of(prompt_seq(a, b).nq) * a.kv_heads;
   int incl = mine;
 #pragma unroll
@@ -384,15 +397,18 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   }
   if (lane == 31) s_warp[warp] = incl;
   if (tid == 0) {
+#pragma unroll 1
     for (int i = 0; i < S; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);  // both issuers
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
+      mbar_init(&turn[i], 1);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_free[i], 4);
     }
@@ -422,6 +438,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       return true;
     }
     int sl = 0;
+#pragma unroll 1
     for (int i = lane; i < kPaThreads; i += 32)
       if (s_sum[i] <= x) sl = i;
     sl = __reduce_max_sync(~0u, sl);
@@ -456,6 +473,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       }
       const uint32_t q_bytes = static_cast<uint32_t>(C::SL * group * tpt * 128);
       int u = 0, qn[2] = {0, 0};
+#pragma unroll 1
       for (int n = 0; item(n, it); ++n) {
         const int blocks = max(it.n[0], it.n[1]);
         if (lane == 0 && !*s_bad) {
@@ -468,6 +486,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
               tma_load_3d(tiles + i * C::TILE + sl * C::SLICE, &maps.q, sl * 64, it.kvh * group, it.s.q0 + it.t0 + i * tpt,
                           &q_full[i]);
           }
+#pragma unroll 1
           for (int j = 0; j < 2 * blocks && !*s_bad; ++j, ++u) {
             const int st = u % S;
             if (u >= S && !mbar_wait_bounded(&kv_empty[st], ((u / S) - 1) & 1, a.err)) {
@@ -484,70 +503,114 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       }
       if (lane == 0 && *s_bad)  // a wait ran out: let the copies in flight land before the CTA leaves
         for (int i = max(u - S, 0); i < u; ++i) mbar_wait_bounded(&kv_full[i % S], (i / S) & 1, a.err);
-    } else if (warp == kPaMma) {
-      // ============================ MMA issuer ================================
+    } else if (warp < kPaMma + 2) {
+      // ==================== MMA issuer of tile i ============================
+      // Runs converged and issues from one lane; descriptors are sums of
+      // precomputed halves, so little stands between two products (with whole
+      // descriptors built for each, one came every 130-170 cycles, not 65).
       constexpr uint32_t kAb = E::is_bf16 ? 1u : 0u;
-      const uint32_t id_s = umma_idesc(kAb, kPaRows, kPaKeys);
-      const uint32_t id_o = umma_idesc(kAb, kPaRows, DP) | kUmmaBMajorN;
-      int u = 0, qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};
-      auto wait = [&](uint64_t* bar, int parity) {
-        if (!*s_bad && !mbar_wait_bounded(bar, parity, a.err)) *s_bad = 1;
-      };
-      auto scores = [&](int i, int st) {
-        const uint32_t qa = smem_u32(tiles + i * C::TILE), ka = smem_u32(ring + st * C::TILE);
-  #pragma unroll
-        for (int sl = 0; sl < C::SL; ++sl) {
-          const uint64_t dq = umma_desc(qa + sl * C::SLICE, 1024, 2), dk = umma_desc(ka + sl * C::SLICE, 1024, 2);
-  #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_f16(tbase + i * kPaKeys, dq + 2 * ks, dk + 2 * ks, id_s, sl > 0 || ks > 0 ? 1u : 0u);
+      constexpr uint32_t id_s = (1u << 4) | (kAb << 7) | (kAb << 10) | ((kPaKeys >> 3) << 17) | ((kPaRows >> 4) << 24);
+      constexpr uint32_t id_o = (1u << 4) | (kAb << 7) | (kAb << 10) | ((DP >> 3) << 17) | ((kPaRows >> 4) << 24) | kUmmaBMajorN;
+      // descriptor halves (see umma_desc): K-major Q and K tiles; V as it lies,
+      // its dimensions contiguous, SLICE bytes between groups of 64 of them
+      constexpr uint32_t hi_d = (1024u >> 4) | (1u << 14) | (2u << 29), lo_k = 1u << 16;
+      constexpr uint32_t lo_v = static_cast<uint32_t>(C::SLICE >> 4) << 16;
+      const uint32_t tm = __shfl_sync(~0u, tbase, 0);
+      const uint32_t q_base = __shfl_sync(~0u, smem_u32(tiles) >> 4, 0), kv_base = q_base + 2 * (C::TILE >> 4);
+      const uint32_t bars = __shfl_sync(~0u, smem_u32(smem), 0);
+      auto bar = [&](const uint64_t* p) { return bars + static_cast<uint32_t>(p - kv_full) * 8; };
+      const int i = __shfl_sync(~0u, warp - kPaMma, 0);
+      const uint32_t ts = tm + i * kPaKeys, to = tm + C::COL_O + i * DP;
+      const uint32_t q_lo = (q_base + i * (C::TILE >> 4)) | lo_k;
+      uint32_t st = 0, ph = 0;  // ring position of the next block
+      uint32_t q_par = 0, p_par = 0, o_par = 1, t_par = i ? 0 : 1;
+      bool ok = true;
+      auto wait = [&](uint32_t at, uint32_t parity) { ok = ok && mbar_wait_warp(at, parity, a.err); };
+      auto next = [&] {
+        if (++st == S) {
+          st = 0;
+          ph ^= 1;
         }
-        umma_commit(&s_full[i]);
       };
-      for (int n = 0; item(n, it); ++n) {
-        const int blocks = max(it.n[0], it.n[1]);
-        if (lane == 0 && blocks > 0) {
-          wait(&kv_full[u % S], (u / S) & 1);  // K(0)
-          tc_fence_after();
-          for (int i = 0; i < 2; ++i)
-            if (it.n[i] > 0 && !*s_bad) {
-              wait(&q_full[i], qn[i]++ & 1);
-              if (!*s_bad) scores(i, u % S);
-              if (it.n[i] == 1) umma_commit(&q_empty[i]);
+#pragma unroll 1
+      for (int n = 0; ok && item(n, it); ++n) {
+        const int mine = __shfl_sync(~0u, i ? it.n[1] : it.n[0], 0);
+        const int blocks = __shfl_sync(~0u, max(it.n[0], it.n[1]), 0);
+        // step j: O_i += P_i(j - 1) V(j - 1), then S_i(j) = Q_i K(j)^T
+        uint32_t v_st = 0;
+#pragma unroll 1
+        for (int j = 0; j <= blocks && blocks > 0 && ok; ++j) {
+          if (j > 0) {
+            v_st = st;
+            wait(bar(kv_full) + 8 * st, ph);  // V(j - 1)
+            next();
+          }
+          const uint32_t k_st = st;
+          if (j < blocks) {
+            wait(bar(kv_full) + 8 * st, ph);  // K(j)
+            next();
+          }
+          const bool pv = j > 0 && j <= mine, qk = j < mine;
+          if (j == 0 && qk) {
+            wait(bar(q_full) + 8 * i, q_par);
+            q_par ^= 1;
+          }
+          if (pv) {
+            if (j == 1) {  // the tile's previous output was read (the first time: nothing to wait for)
+              wait(bar(o_free) + 8 * i, o_par);
+              o_par ^= 1;
             }
-          umma_commit(&kv_empty[u % S]);
-          for (int j = 0; j < blocks && !*s_bad; ++j) {
-            const int sv = (u + 1) % S, sk = (u + 2) % S;
-            wait(&kv_full[sv], ((u + 1) / S) & 1);  // V(j)
-            if (j + 1 < blocks) wait(&kv_full[sk], ((u + 2) / S) & 1);  // K(j + 1)
-            for (int i = 0; i < 2; ++i) {
-              if (j >= it.n[i] || *s_bad) continue;
-              if (j == 0 && on[i]++ > 0) wait(&o_free[i], on[i] & 1);  // the tile's previous output was read
-              wait(&p_full[i], pn[i]++ & 1);
-              if (*s_bad) continue;
-              tc_fence_after();
-              const uint32_t va = smem_u32(ring + sv * C::TILE);
-  #pragma unroll
-              for (int ks = 0; ks < kPaKeys / 16; ++ks)
-                umma_f16_ts(tbase + C::COL_O + i * DP, tbase + i * kPaKeys + ks * 8,
-                            umma_desc_mn(va + ks * 2048, C::SLICE, 1024), id_o, j > 0 || ks > 0 ? 1u : 0u);
-              if (j + 1 < it.n[i]) {
-                scores(i, sk);
-                if (j + 2 == it.n[i]) umma_commit(&q_empty[i]);
-              } else {
-                umma_commit(&o_full[i]);
+          }
+          const uint32_t v_lo = (kv_base + v_st * (C::TILE >> 4)) | lo_v, k_lo = (kv_base + k_st * (C::TILE >> 4)) | lo_k;
+          auto weighted = [&](int h) {  // O_i += P_i V for half of the keys
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              umma_f16_ts_lo(to, ts + h * 32 + ks * 8, v_lo + h * 512 + ks * 128, hi_d, id_o, ks + h > 0 || j > 1 ? 1u : 0u);
+          };
+          if (pv) {
+            wait(bar(p_full) + 16 * i, p_par);
+            tc_fence_after();
+            if (ok && elect_one()) weighted(0);
+            __syncwarp();
+          }
+          wait(bar(turn) + 8 * i, t_par);
+          t_par ^= 1;
+          if (pv) {
+            wait(bar(p_full) + 16 * i + 8, p_par);
+            p_par ^= 1;
+          }
+          tc_fence_after();
+          if (ok && elect_one()) {
+            if (pv) {
+              weighted(1);
+              if (!qk) {
+                umma_commit_at(bar(o_full) + 8 * i);
+                mbar_arrive(turn + 1 - i);
               }
             }
-            umma_commit(&kv_empty[sv]);
-            if (j + 1 < blocks) umma_commit(&kv_empty[sk]);
-            u += 2;
+            if (qk) {
+#pragma unroll
+              for (int ks = 0; ks < DP / 16; ++ks) {
+                const uint32_t at = (ks >> 2) * (C::SLICE >> 4) + 2 * (ks & 3);
+                umma_f16_lo(ts, q_lo + at, hi_d, k_lo + at, hi_d, id_s, ks > 0 ? 1u : 0u);
+              }
+              umma_commit_at(bar(s_full) + 8 * i);
+              mbar_arrive(turn + 1 - i);
+              if (j + 1 == mine) umma_commit_at(bar(q_empty) + 8 * i);
+            }
+            if (!pv && !qk) mbar_arrive(turn + 1 - i);
+            if (j > 0) umma_commit_at(bar(kv_empty) + 8 * v_st);
+            if (j < blocks) umma_commit_at(bar(kv_empty) + 8 * k_st);
           }
+          __syncwarp();
         }
-        __syncwarp();
       }
-      if (lane == 0 && *s_bad) {  // let the products in flight end before TMEM is freed
-        umma_commit(&o_full[0]);
-        mbar_wait_bounded(&o_full[0], 0, a.err, 1000000ull);
+      if (!ok) {
+        // a wait ran out: stop the others, and let the products in flight end
+        // before TMEM is freed
+        *s_bad = 1;
+        if (elect_one()) umma_commit_at(bar(o_full) + 8 * i);
+        mbar_wait_bounded(o_full + i, 0, a.err, 1000000ull);
       }
     }
   } else {
@@ -558,7 +621,8 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     const uint32_t to = tbase + C::COL_O + i * DP + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float sc = a.scale * kLog2e;
     int sn = 0, on = 0;
-    for (int n = 0; item(n, it) && !*s_bad; ++n) {
+#pragma unroll 1
+    for (int n = 0; item(n, it) && __all_sync(~0u, !*s_bad); ++n) {
       const int first = it.t0 + i * tpt;
       const int blocks = i ? it.n[1] : it.n[0];
       if (blocks < 0 || first >= it.s.nq) continue;
@@ -567,76 +631,97 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       const int shift = it.s.nk - it.s.nq + 1;
       const int lim = min(token + shift, it.s.nk);  // keys this row sees
       float m = -INFINITY, l = 0.f;
+#pragma unroll 1
       for (int j = 0; j < blocks; ++j) {
-        if (!mbar_wait_bounded(&s_full[i], sn++ & 1, a.err)) {
+        if (!mbar_wait_warp(smem_u32(&s_full[i]), sn++ & 1, a.err)) {
           *s_bad = 1;
           break;
         }
         tc_fence_after();
         uint32_t x[4][32];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32_nowait(ts + q * 32, x[q]);
-        tmem_wait_ld();
-        if ((j + 1) * kPaKeys > first + shift) {  // some row of the tile sees less than the whole block
-          const int left = lim - j * kPaKeys;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
+        tmem_ld32_nowait(ts, x[0]);
+        tmem_ld32_nowait(ts + 32, x[1]);
+        tmem_wait_ld32(x[0]);
+        tmem_wait_ld32(x[1]);
+        tmem_ld32_nowait(ts + 64, x[2]);
+        tmem_ld32_nowait(ts + 96, x[3]);
+        const int left = lim - j * kPaKeys;
+        const bool masked = (j + 1) * kPaKeys > first + shift;  // some row of the tile sees less than the whole block
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto row_max = [&](uint32_t(&y)[32], int at) {
+          if (masked) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (q * 32 + e >= left) x[q][e] = 0xff800000u;
-        }
-        float t[4];
+              if (at + e >= left) y[e] = 0xff800000u;
+          }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          t[q] = __uint_as_float(x[q][0]);
-#pragma unroll
-          for (int e = 1; e < 32; ++e) t[q] = fmaxf(t[q], __uint_as_float(x[q][e]));
-        }
-        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          for (int e = 0; e < 32; e += 2)
+            t[e / 2 % 4] = max3(t[e / 2 % 4], __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
+        };
+        row_max(x[0], 0);
+        row_max(x[1], 32);
+        tmem_wait_ld32(x[2]);
+        tmem_wait_ld32(x[3]);
+        row_max(x[2], 64);
+        row_max(x[3], 96);
+        const float top = max3(max3(t[0], t[1], t[2]), t[3], -INFINITY);
         if (__any_sync(~0u, (top - m) * sc > kPaLazy || (m == -INFINITY && top > m))) {
           const float mn = fmaxf(m, top);
           const float f = m == -INFINITY ? 0.f : ex2((m - mn) * sc);
           m = mn;
           l *= f;
           if (j > 0) {
-#pragma unroll
+#pragma unroll 1
             for (int q = 0; q < DP / 32; ++q) {
               uint32_t o[32];
               tmem_ld32_nowait(to + q * 32, o);
-              tmem_wait_ld();
+              tmem_wait_ld32(o);
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
               tmem_st32_nowait(to + q * 32, o);
             }
           }
         }
+        if (!(top < INFINITY)) l = NAN;  // NaN and infinite scores: the polynomial would lose them
         const float off = m == -INFINITY ? 0.f : -m * sc;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t sc2 = pack_f2(sc, sc), off2 = pack_f2(off, off);
+        uint64_t sum[2] = {0, 0};
+        // 64 keys at a time, so that the second product starts on the first half
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t p[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float p0 = ex2(fmaf(__uint_as_float(x[2 * h + e / 16][(2 * e) % 32]), sc, off));
-            const float p1 = ex2(fmaf(__uint_as_float(x[2 * h + e / 16][(2 * e) % 32 + 1]), sc, off));
-            sum[e & 1] += p0;
-            sum[2 + (e & 1)] += p1;
+            const uint32_t* y = &x[2 * h + e / 16][(2 * e) % 32];
+            const uint64_t z = fma_f2(pack_f2(__uint_as_float(y[0]), __uint_as_float(y[1])), sc2, off2);
+            float p0, p1;
+            if (e % 8 < kPaFma) {
+              ex2_fma2(z, p0, p1);
+            } else {
+              unpack_f2(z, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+            }
+            sum[e & 1] = add_f2(sum[e & 1], pack_f2(p0, p1));
             p[e] = E::pack2(p0, p1);
           }
           tmem_st32_nowait(ts + h * 32, p);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[i]);
+        float l0, l1;
+        unpack_f2(add_f2(sum[0], sum[1]), l0, l1);
+        l += l0 + l1;
       }
+      if (m == -INFINITY && l == l) l = 0.f;  // no key seen (the polynomial's smallest value is not 0)
       // ---- the tile's output
       const int64_t at = static_cast<int64_t>(it.s.q0 + token) * a.heads + head;
       T* op = static_cast<T*>(a.out) + at * a.dim;
       bool odd = false;
       if (blocks > 0) {
-        if (*s_bad || !mbar_wait_bounded(&o_full[i], on++ & 1, a.err)) {
+        if (__any_sync(~0u, *s_bad) || !mbar_wait_warp(smem_u32(&o_full[i]), on++ & 1, a.err)) {
           *s_bad = 1;
           break;
         }
@@ -646,7 +731,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         for (int q = 0; q < DP / 32; ++q) {
           uint32_t o[32];
           tmem_ld32_nowait(to + q * 32, o);
-          tmem_wait_ld();
+          tmem_wait_ld32(o);
           if (q == DP / 32 - 1) {
             tc_fence_before();
             __syncwarp();
@@ -666,6 +751,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           }
         }
       } else if (live) {  // no row of the tile sees a key
+#pragma unroll 1
         for (int d = 0; d < a.dim; d += 8) *reinterpret_cast<uint4*>(op + d) = make_uint4(0, 0, 0, 0);
       }
       if (a.lse && live) a.lse[at] = l == 0.f ? -INFINITY : (m * sc + __log2f(l)) * kLn2;

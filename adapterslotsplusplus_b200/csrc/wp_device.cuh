@@ -86,6 +86,26 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// The same for a converged warp, all of whose lanes get the same answer (bar: a
+// shared-memory address), in few instructions: at most 2^20 polls, each of
+// which sleeps up to 1 us.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int* err) {
+  uint32_t ok;
+#pragma unroll 1
+  for (int n = 1 << 20; n; --n) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(1000u)
+        : "memory");
+    if (__all_sync(~0u, ok)) return true;
+  }
+  if (err) atomicOr(err, kErrWaitTimeout);
+  return false;
+}
+
 // ---- flags shared with other GPUs (peer memory) ---------------------------
 
 __device__ __forceinline__ int ld_acquire_sys(const int* p) {
@@ -234,6 +254,18 @@ __device__ __forceinline__ uint32_t sw128(int row, int col) {
 
 __device__ __forceinline__ void named_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
+// named_sync that also tells whether `v` holds in any of the threads.
+__device__ __forceinline__ bool named_sync_or(int id, int nthreads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(nthreads), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -449,28 +481,39 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
       : "memory");
 }
 
-// The same with A (16-bit, two consecutive K elements per column) in TMEM.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      :
+      : "memory");
+  return r != 0;
+}
+
+// Products with descriptors in halves: the low one moves along K by additions,
+// the high one is a constant.
+__device__ __forceinline__ void umma_f16_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A in TMEM: 16-bit, two consecutive K elements per column.
+__device__ __forceinline__ void umma_f16_ts_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
-// Descriptor of an operand tile whose M / N dimension is contiguous ([K rows][64
-// elements = 128 bytes], 128-byte swizzle): `lbo` bytes between groups of 64
-// M / N elements, `sbo` bytes between groups of 8 K rows.
-__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
-  d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;
-  d |= static_cast<uint64_t>(2u) << 61;
-  return d;
-}
 // Instruction descriptor bit: B's N dimension is the contiguous one.
 constexpr uint32_t kUmmaBMajorN = 1u << 16;
 
@@ -478,6 +521,11 @@ constexpr uint32_t kUmmaBMajorN = 1u << 16;
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
+}
+
+// umma_commit to a shared-memory address.
+__device__ __forceinline__ void umma_commit_at(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // Each lane of the warp reads 16 consecutive fp32 columns of its TMEM lane.
@@ -520,6 +568,24 @@ __device__ __forceinline__ void tmem_st32_nowait(uint32_t taddr, const uint32_t 
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Writes 16 columns; complete it with tmem_wait_st().
+__device__ __forceinline__ void tmem_st16_nowait(uint32_t taddr, const float (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+      : "memory");
+}
+// Completes the reads issued so far and holds uses of r back until then.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Each lane of the warp reads 32 consecutive fp32 columns of its TMEM lane.
@@ -696,6 +762,57 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 values in one 64-bit register: one instruction for both.
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// NaN if any is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^t for two values t <= 127 on the FMA pipe, for kernels whose special-
+// function unit is the bottleneck: t = n + f with n the nearest integer (added
+// and taken away again as 1.5 * 2^23 + n, whose low bits are n), 2^f on [-1/2,
+// 1/2] by the degree-4 polynomial of least relative error (2.6e-6; Remez
+// exchange), n added to its exponent. Below 2^-126 the result is about 0; NaN
+// does not survive.
+__device__ __forceinline__ void ex2_fma2(uint64_t t, float& lo, float& hi) {
+  constexpr float kMagic = 12582912.f;
+  float a, b;
+  unpack_f2(t, a, b);
+  t = pack_f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t z = add_f2(t, pack_f2(kMagic, kMagic));
+  const uint64_t f = add_f2(t, fma_f2(z, pack_f2(-1.f, -1.f), pack_f2(kMagic, kMagic)));
+  uint64_t p = pack_f2(0.009570102207362652f, 0.009570102207362652f);
+  p = fma_f2(p, f, pack_f2(0.05591785907745361f, 0.05591785907745361f));
+  p = fma_f2(p, f, pack_f2(0.240247443318367f, 0.240247443318367f));
+  p = fma_f2(p, f, pack_f2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma_f2(p, f, pack_f2(0.9999992847442627f, 0.9999992847442627f));
+  float zl, zh, pl, ph;
+  unpack_f2(z, zl, zh);
+  unpack_f2(p, pl, ph);
+  lo = __uint_as_float(__float_as_uint(pl) + (__float_as_uint(zl) << 23));
+  hi = __uint_as_float(__float_as_uint(ph) + (__float_as_uint(zh) << 23));
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
