@@ -7,17 +7,19 @@
 //   rank         = 1 + #(x > x_token)
 //   alternatives: the `top` largest logits, equal ones by ascending index
 //
-// x - M comes first and is exact for the values that matter, so neither a
-// large common offset nor rows of the type's lowest value lose anything. A
-// logit of minus infinity has probability 0; a row of nothing else is empty:
+// A logit of minus infinity has probability 0; a row of nothing else is empty:
 // log probabilities -inf, entropy 0. NaN and plus infinity make a row NaN.
 //
-// What bounds it: T * V logits from HBM once; in 16 bits the instructions per
-// logit (7-8 of the 11 that fit in its time at the memory rate) come close
-// behind. The row is read a second time, from L2, for the alternatives only:
-// every thread's own maximum is known after the first pass, so the top-th
-// largest of those is a lower bound that at least `top` logits reach and few
-// others do.
+// What bounds it: T * V logits from HBM once, and close behind it in 16 bits
+// the instructions per logit (6.5 of the 11 that fit into its time at the
+// memory rate). So the pass works in log2 units, where e^(x - M) is one fused
+// multiply-add and one 2^y, with a running reference R = fl(M log2 e): its own
+// rounding is the same for every logit and is taken out of the results again
+// (`residue`). The row is not read a second time for the alternatives: after
+// the pass every thread knows its own maximum, the top-th largest of 32 groups'
+// maxima is a bound that at least `top` logits reach and few others do, and
+// only the threads whose maximum reaches it look at their logits again (a warp
+// together for each).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -32,8 +34,16 @@
 namespace wp {
 namespace {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
+#ifndef LP_PER
+#define LP_PER 4
+#endif
+constexpr int kLpPerSm = LP_PER;  // CTAs of one SM
 constexpr int kLpWarps = kLpThreads / 32;
+#ifndef LP_AHEAD
+#define LP_AHEAD 4
+#endif
+constexpr int kLpAhead = LP_AHEAD;  // vectors that a thread has in flight
 constexpr int kLpCands = 1024;  // candidates for the alternatives in one CTA
 
 // 16 bytes of logits as fp32.
@@ -41,6 +51,22 @@ template <typename T>
 struct Vec {
   static constexpr int N = 8;
   static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);  // NaN if either is
+  // The lowest logit that the fast pass tells from minus infinity; a part of a
+  // row whose maximum is not well above it takes the exact pass.
+  static constexpr float kLow = Elem<T>::is_bf16 ? -0x1p126f : -65504.f;
+  static constexpr uint32_t kNone = Elem<T>::is_bf16 ? 0xff80ff80u : 0xfc00fc00u;  // minus infinity
+  static constexpr uint32_t kLow2 = Elem<T>::is_bf16 ? 0xfe80fe80u : 0xfbfffbffu;
+  // -1 in each half that is above the same half of g
+  static __device__ __forceinline__ uint32_t above2(uint32_t v, uint32_t g);
+  static __device__ __forceinline__ int above(const uint4& v, uint32_t g2, float) {
+    int n = __dp4a(static_cast<int>(above2(v.x, g2)), 0x00010001, 0);
+    n = __dp4a(static_cast<int>(above2(v.y, g2)), 0x00010001, n);
+    n = __dp4a(static_cast<int>(above2(v.z, g2)), 0x00010001, n);
+    return -__dp4a(static_cast<int>(above2(v.w, g2)), 0x00010001, n);
+  }
+  static __device__ __forceinline__ uint4 raised(const uint4& v) {
+    return make_uint4(max2(v.x, kLow2), max2(v.y, kLow2), max2(v.z, kLow2), max2(v.w, kLow2));
+  }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -70,8 +96,30 @@ __device__ __forceinline__ uint32_t Vec<__half>::max2(uint32_t a, uint32_t b) {
   return r;
 }
 template <>
+__device__ __forceinline__ uint32_t Vec<__nv_bfloat16>::above2(uint32_t v, uint32_t g) {
+  return __hgt2_mask(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<__nv_bfloat162*>(&g));
+}
+template <>
+__device__ __forceinline__ uint32_t Vec<__half>::above2(uint32_t v, uint32_t g) {
+  return __hgt2_mask(*reinterpret_cast<__half2*>(&v), *reinterpret_cast<__half2*>(&g));
+}
+template <>
 struct Vec<float> {
   static constexpr int N = 4;
+  static constexpr float kLow = -0x1p126f;
+  static constexpr uint32_t kNone = 0xff800000u;
+  static __device__ __forceinline__ int above(const uint4& v, uint32_t, float g) {
+    return (__uint_as_float(v.x) > g) + (__uint_as_float(v.y) > g) + (__uint_as_float(v.z) > g) + (__uint_as_float(v.w) > g);
+  }
+  static __device__ __forceinline__ float raised1(uint32_t v) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(v)), "f"(kLow));
+    return r;
+  }
+  static __device__ __forceinline__ uint4 raised(const uint4& v) {
+    return make_uint4(__float_as_uint(raised1(v.x)), __float_as_uint(raised1(v.y)), __float_as_uint(raised1(v.z)),
+                      __float_as_uint(raised1(v.w)));
+  }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
   }
@@ -107,21 +155,21 @@ __device__ __forceinline__ unsigned long long key_of(float x, int index) {
 }
 
 struct Stat {
-  float m;  // maximum (at least -FLT_MAX: a reference that is always finite)
-  float l;  // sum e^(x - m)
-  float s;  // sum e^(x - m) (x - m)
-  int above;  // logits above the given one
   float raw;  // maximum, -inf while there is none
+  float r2;  // reference in log2 units, about raw * log2 e
+  float l;  // sum 2^(x log2 e - r2)
+  float s;  // sum 2^(x log2 e - r2) (x log2 e - r2)
+  int above;  // logits above the given one
 };
 
 __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
   Stat r;
-  r.m = fmaxf(a.m, b.m);
   r.raw = fmaxf(a.raw, b.raw);
+  r.r2 = fmaxf(a.r2, b.r2);
   r.above = a.above + b.above;
   // a side that is far below contributes 0, not 0 * infinity
-  const float da = fmaxf(a.m - r.m, -1e4f), db = fmaxf(b.m - r.m, -1e4f);
-  const float fa = ex2(da * kLog2e), fb = ex2(db * kLog2e);
+  const float da = fmaxf(a.r2 - r.r2, -1e4f), db = fmaxf(b.r2 - r.r2, -1e4f);
+  const float fa = ex2(da), fb = ex2(db);
   r.l = fa * a.l + fb * b.l;
   r.s = fa * fmaf(a.l, da, a.s) + fb * fmaf(b.l, db, b.s);
   return r;
@@ -129,170 +177,241 @@ __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
 
 __device__ __forceinline__ Stat shfl_xor(const Stat& a, int o) {
   Stat r;
-  r.m = __shfl_xor_sync(~0u, a.m, o);
+  r.raw = __shfl_xor_sync(~0u, a.raw, o);
+  r.r2 = __shfl_xor_sync(~0u, a.r2, o);
   r.l = __shfl_xor_sync(~0u, a.l, o);
   r.s = __shfl_xor_sync(~0u, a.s, o);
   r.above = __shfl_xor_sync(~0u, a.above, o);
-  r.raw = __shfl_xor_sync(~0u, a.raw, o);
   return r;
 }
 
 // What one CTA of a row's cluster hands to the first one.
 struct alignas(16) Share {
   Stat stat;
-  unsigned long long top[kMaxTop];
+  alignas(16) unsigned long long top[kMaxTop];  // descending, 0 past the last
 };
 
-// Elements of one row that this CTA visits: f(x, index) for the unaligned
+// Where the 16-byte vectors of a row start and end.
+template <typename T>
+struct Row {
+  const T* p;
+  int vocab, head, nvec, tail;
+  __device__ __forceinline__ Row(const T* row, int v) : p(row), vocab(v) {
+    head = min(static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)), vocab);
+    nvec = (vocab - head) / Vec<T>::N;
+    tail = head + nvec * Vec<T>::N;
+  }
+  __device__ __forceinline__ uint4 vec(int i) const { return __ldg(reinterpret_cast<const uint4*>(p + head) + i); }
+};
+
+// Elements of one row that this thread visits: f(x, index) for the unaligned
 // head and tail, g(vector, first index) for the 16-byte vectors between.
 template <typename T, typename F, typename G>
-__device__ __forceinline__ void for_row(const T* row, int vocab, int rank, int ranks, F&& f, G&& g) {
+__device__ __forceinline__ void for_row(const Row<T>& row, int rank, int ranks, F&& f, G&& g) {
   constexpr int N = Vec<T>::N;
-  const int head = min(static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)), vocab);
-  const int nvec = (vocab - head) / N;
-  const int tail = head + nvec * N;
-  const uint4* v = reinterpret_cast<const uint4*>(row + head);
   const int step = ranks * kLpThreads;
+  // the next kLpAhead vectors load while these are worked on; those past the
+  // end count as minus infinity
+  uint4 x[kLpAhead];
+  auto load = [&](int i, bool inside) {
+#pragma unroll
+    for (int j = 0; j < kLpAhead; ++j)
+      x[j] = inside || i + j * step < row.nvec ? row.vec(i + j * step)
+                                               : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+  };
   int i = rank * kLpThreads + threadIdx.x;
-  // four loads in flight
-  for (; i + 3 * step < nvec; i += 4 * step) {
-    uint4 x[4];
+  load(i, false);
+  auto work = [&](bool inside) {
+    uint4 y[kLpAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = __ldg(v + i + j * step);
+    for (int j = 0; j < kLpAhead; ++j) y[j] = x[j];
+    load(i + kLpAhead * step, inside);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g(x[j], head + (i + j * step) * N);
-  }
-  for (; i < nvec; i += step) g(__ldg(v + i), head + i * N);
+    for (int j = 0; j < kLpAhead; ++j) g(y[j], row.head + (i + j * step) * N);
+    i += kLpAhead * step;
+  };
+#pragma unroll 1
+  while (i + (2 * kLpAhead - 1) * step < row.nvec) work(true);
+#pragma unroll 1
+  while (i < row.nvec) work(false);
   if (rank == ranks - 1) {
     const int t = threadIdx.x;
-    if (t < head) f(load1(row + t), t);
-    if (tail + t < vocab) f(load1(row + tail + t), tail + t);
+    if (t < row.head) f(load1(row.p + t), t);
+    if (row.tail + t < row.vocab) f(load1(row.p + row.tail + t), row.tail + t);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(const LogprobArgs a) {
   constexpr int N = Vec<T>::N;
   __shared__ Stat s_stat[kLpWarps];
   __shared__ uint32_t s_max[kLpThreads];  // each thread's maximum
-  __shared__ unsigned long long s_cand[kLpCands];
-  __shared__ int s_ncand;
+  __shared__ unsigned long long s_cand[kLpCands], s_top[kMaxTop], s_best[kLpWarps];
+  __shared__ uint16_t s_hit[kLpThreads];
+  __shared__ int s_ncand, s_nhit;
   __shared__ uint32_t s_bound;
-  __shared__ unsigned long long s_best[kLpWarps];
   __shared__ Share s_share[8];  // on the cluster's first CTA: every CTA's result
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
   if (ranks > 1) cluster_arrive();  // every CTA runs before the first one's shared memory is written
   const int64_t t = blockIdx.x / ranks;
-  const T* row = static_cast<const T*>(a.logits) + t * a.ld;
+  const Row<T> row(static_cast<const T*>(a.logits) + t * a.ld, a.vocab);
 
   const long long token = a.tokens64 ? __ldg(static_cast<const long long*>(a.tokens) + t)
                                      : static_cast<long long>(__ldg(static_cast<const int*>(a.tokens) + t));
   const bool known = token >= 0 && token < a.vocab;
-  const float given = known ? load1(row + token) : -INFINITY;
+  const float given = known ? load1(row.p + token) : -INFINITY;
 
-  // ---- pass 1: running maximum, sums, rank
-  Stat st{-FLT_MAX, 0.f, 0.f, 0, -INFINITY};
-  auto add = [&](float x) {
-    // x - m, kept finite where x is far below (minus infinity has e^(x - m)
-    // = 0 and adds 0 to both sums); NaN stays NaN
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x - st.m), "f"(-1e38f));
-    const float e = ex2(d * kLog2e);
-    st.l += e;
-    st.s = fmaf(e, d, st.s);
-  };
+  uint32_t given2 = 0;
+  if constexpr (sizeof(T) == 2) given2 = Elem<T>::pack2(given, given);
+
+  // ---- the pass: running maximum, sums, rank
+  Stat st{-INFINITY, Vec<T>::kLow * kLog2e, 0.f, 0.f, 0};
+  uint64_t l2 = 0, s2 = 0, neg2 = pack_f2(-st.r2, -st.r2);  // sums of even and odd elements; -r2 twice
+  const uint64_t log2e2 = pack_f2(kLog2e, kLog2e);
   auto raise = [&](float x) {
     st.raw = fmaxf(st.raw, x);
-    const float m = fmaxf(st.m, x), d = fmaxf(st.m - m, -1e4f), f = ex2(d * kLog2e);
-    st.s = f * fmaf(st.l, d, st.s);
-    st.l *= f;
-    st.m = m;
+    const float r2 = fmaxf(st.r2, x * kLog2e), d = fmaxf(st.r2 - r2, -1e30f), f = ex2(d);  // 0 * finite
+    const uint64_t f2 = pack_f2(f, f);
+    s2 = fma_f2(f2, fma_f2(l2, pack_f2(d, d), s2), 0);
+    l2 = fma_f2(f2, l2, 0);
+    st.r2 = r2;
+    neg2 = pack_f2(-r2, -r2);
+  };
+  auto add2 = [&](float x, float y) {
+    const uint64_t d = fma_f2(pack_f2(x, y), log2e2, neg2);
+    float d0, d1;
+    unpack_f2(d, d0, d1);
+    const uint64_t e = pack_f2(ex2(d0), ex2(d1));
+    l2 = add_f2(l2, e);
+    s2 = fma_f2(e, d, s2);
   };
   for_row(
-      row, a.vocab, rank, ranks,
+      row, rank, ranks,
       [&](float x, int) {
         if (x > st.raw) raise(x);
-        add(x);
         st.above += x > given;
+        add2(x == x ? fmaxf(x, Vec<T>::kLow) : x, Vec<T>::kLow);
       },
       [&](const uint4& v, int) {
         float x[N];
-        Vec<T>::unpack(v, x);
         const float top = Vec<T>::largest(v);
         if (top > st.raw) raise(top);
-        if (top > given) {
+        if (top > given) st.above += Vec<T>::above(v, given2, given);
+        Vec<T>::unpack(Vec<T>::raised(v), x);
 #pragma unroll
-          for (int i = 0; i < N; ++i) st.above += x[i] > given;
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) add(x[i]);
+        for (int i = 0; i < N; i += 2) add2(x[i], x[i + 1]);
       });
-  s_max[tid] = st.raw == -INFINITY ? 0u : ordered(st.raw);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) st = merge(st, shfl_xor(st, o));
-  if (lane == 0) s_stat[warp] = st;
-  if (tid == 0) s_ncand = 0;
-  __syncthreads();
-  if (warp == 0) {
-    Stat w = lane < kLpWarps ? s_stat[lane] : Stat{-FLT_MAX, 0.f, 0.f, 0, -INFINITY};
-#pragma unroll
-    for (int o = kLpWarps / 2; o; o >>= 1) w = merge(w, shfl_xor(w, o));
-    if (lane == 0) s_stat[0] = w;
-  } else if (warp == 1 && a.top > 0) {
-    // top-th largest of the threads' maxima (0: fewer than that have one)
-    uint32_t k[kLpThreads / 32];
-#pragma unroll
-    for (int i = 0; i < kLpThreads / 32; ++i) k[i] = s_max[i * 32 + lane];
-    uint32_t best = 0;
-    for (int n = 0; n < a.top; ++n) {
-      uint32_t mine = 0;
-#pragma unroll
-      for (int i = 0; i < kLpThreads / 32; ++i) mine = max(mine, k[i]);
-      best = __reduce_max_sync(~0u, mine);
-      const int owner = __ffs(__ballot_sync(~0u, mine == best)) - 1;
-      if (lane == owner) {
-        bool gone = false;
-#pragma unroll
-        for (int i = 0; i < kLpThreads / 32; ++i)
-          if (!gone && k[i] == best) {
-            k[i] = 0;
-            gone = true;
-          }
-      }
-    }
-    if (lane == 0) s_bound = best;
+  {
+    float p, q;
+    unpack_f2(l2, p, q);
+    st.l = p + q;
+    unpack_f2(s2, p, q);
+    st.s = p + q;
   }
+  const bool nan = st.l != st.l;
+  s_max[tid] = st.raw == -INFINITY ? 0u : ordered(st.raw);
+  const uint32_t my_max = nan ? 0xffffffffu : s_max[tid];
+  Stat w = st;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) w = merge(w, shfl_xor(w, o));
+  if (lane == 0) s_stat[warp] = w;
+  if (tid == 0) s_ncand = s_nhit = 0;
   __syncthreads();
+  if (a.top > 0 && warp == 0) {
+    // 32 groups of threads: the top-th largest of their maxima (0: fewer have one)
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kLpWarps; ++i) mine = max(mine, s_max[i * 32 + lane]);
+    int place = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const uint32_t o = __shfl_sync(~0u, mine, i);
+      place += o > mine || (o == mine && i < lane);
+    }
+    if (place == a.top - 1) s_bound = mine;
+  }
+  w = s_stat[0];
+#pragma unroll
+  for (int i = 1; i < kLpWarps; ++i) w = merge(w, s_stat[i]);
+  // Where nothing is well above the lowest logit (masked rows), or the maximum
+  // is enormous, the sums again with x - M exact: M is known now.
+  if (!(w.raw > Vec<T>::kLow + 200.f && w.raw < 1e38f) && w.raw < INFINITY && w.l == w.l) {
+    float l = 0.f, s = 0.f;
+    const float m = fmaxf(w.raw, -FLT_MAX);
+    auto exact = [&](float x) {
+      const float d = fmaxf((x - m) * kLog2e, -1e30f), e = ex2(d);
+      l += e;
+      s = fmaf(e, d, s);
+    };
+    for_row(
+        row, rank, ranks, [&](float x, int) { exact(x); },
+        [&](const uint4& v, int) {
+          float x[N];
+          Vec<T>::unpack(v, x);
+#pragma unroll
+          for (int i = 0; i < N; ++i) exact(x[i]);
+        });
+    __syncthreads();  // s_stat was read
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      l += __shfl_xor_sync(~0u, l, o);
+      s += __shfl_xor_sync(~0u, s, o);
+    }
+    if (lane == 0) s_stat[warp].l = l, s_stat[warp].s = s;
+    __syncthreads();
+    w.r2 = fminf(fmaxf(m * kLog2e, -3e38f), 3e38f);
+    w.l = w.s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kLpWarps; ++i) w.l += s_stat[i].l, w.s += s_stat[i].s;
+    if (fabsf(m) < 1e37f) {  // relative to the rounded reference, as everywhere else
+      const float d = fmaf(m, kLog2e, -w.r2), f = ex2(d);
+      w.s = f * fmaf(w.l, d, w.s);
+      w.l *= f;
+    }
+  }
 
-  // ---- pass 2: the largest `top` of this CTA's part of the row
+  // ---- the largest `top` of this CTA's part of the row
   unsigned long long mine = 0;  // thread i < top: the i-th largest key
   if (a.top > 0) {
-    const float bound = s_bound == 0 ? -INFINITY : unordered(s_bound);
+    if (tid < kMaxTop) s_top[tid] = 0;
+    __syncthreads();
+    const uint32_t bound = s_bound;
+    const float low = bound == 0 ? -INFINITY : unordered(bound);
     auto keep = [&](float x, int i) {
-      if (!(x < bound)) {
+      if (!(x < low)) {
         const int at = atomicAdd(&s_ncand, 1);
         if (at < kLpCands) s_cand[at] = key_of(x, i);
       }
     };
-    for_row(row, a.vocab, rank, ranks, keep, [&](const uint4& v, int i0) {
-      if (!(Vec<T>::largest(v) < bound)) {
+    // the threads to look at again, each with `per` vectors and perhaps an
+    // element of the row's head and tail; all threads share the work
+    if (my_max >= bound) s_hit[atomicAdd(&s_nhit, 1)] = static_cast<uint16_t>(tid);
+    __syncthreads();
+    const int step = ranks * kLpThreads, per = (row.nvec + step - 1) / step, hits = s_nhit;
+#pragma unroll 4
+    for (int i = tid; i < hits * per; i += kLpThreads) {
+      const int at = rank * kLpThreads + s_hit[i % hits] + i / hits * step;
+      const uint4 v = at < row.nvec ? row.vec(at) : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+      if (at < row.nvec && !(Vec<T>::largest(v) < low)) {
         float x[N];
         Vec<T>::unpack(v, x);
 #pragma unroll
-        for (int i = 0; i < N; ++i) keep(x[i], i0 + i);
+        for (int j = 0; j < N; ++j) keep(x[j], row.head + at * N + j);
       }
-    });
+    }
+    if (rank == ranks - 1 && my_max >= bound) {
+      if (tid < row.head) keep(load1(row.p + tid), tid);
+      if (row.tail + tid < row.vocab) keep(load1(row.p + row.tail + tid), row.tail + tid);
+    }
     __syncthreads();
     const int n = s_ncand;
     if (n <= kLpCands) {
       // a candidate's place is the number of larger keys
-      __shared__ unsigned long long s_top[kMaxTop];
-      if (tid < kMaxTop) s_top[tid] = 0;
-      __syncthreads();
       for (int i = tid; i < n; i += kLpThreads) {
         const unsigned long long k = s_cand[i];
         int place = 0;
+#pragma unroll 4
         for (int j = 0; j < n; ++j) place += s_cand[j] > k;
         if (place < a.top) s_top[place] = k;
       }
@@ -301,13 +420,14 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     } else {
       // long runs of equal logits: one pass over the row for each place
       unsigned long long last = ~0ull;
+#pragma unroll 1
       for (int p = 0; p < a.top; ++p) {
         unsigned long long b = 0;
         auto look = [&](float x, int i) {
           const unsigned long long k = key_of(x, i);
           if (k < last && k > b) b = k;
         };
-        for_row(row, a.vocab, rank, ranks, look, [&](const uint4& v, int i0) {
+        for_row(row, rank, ranks, look, [&](const uint4& v, int i0) {
           float x[N];
           Vec<T>::unpack(v, x);
 #pragma unroll
@@ -331,29 +451,31 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     cluster_wait();
     const uint32_t dst = mapa(smem_u32(&s_share[rank]), 0);
     if (tid == 0) {
-      const Stat w = s_stat[0];
-      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(w.m), "f"(w.l), "f"(w.s),
-                   "f"(__int_as_float(w.above))
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(w.raw), "f"(w.r2), "f"(w.l), "f"(w.s)
                    : "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 16), "f"(w.raw) : "memory");
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 16), "r"(w.above) : "memory");
     }
-    if (tid < a.top)
+    if (tid < kMaxTop)
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(
                        dst + static_cast<uint32_t>(offsetof(Share, top)) + 8u * tid),
                    "l"(mine)
                    : "memory");
     cluster_sync_hw();
     if (rank != 0) return;
+    w = s_share[0].stat;
+    for (int i = 1; i < ranks; ++i) w = merge(w, s_share[i].stat);
   }
-  Stat r = ranks > 1 ? s_share[0].stat : s_stat[0];
-  for (int i = 1; i < ranks; ++i) r = merge(r, s_share[i].stat);
-  const bool empty = r.raw == -INFINITY && r.l == 0.f;
-  const float log_l = logf(r.l);
-  auto log_prob = [&](float x) { return x == -INFINITY && r.l == r.l ? -INFINITY : (x - r.m) - log_l; };
+  const bool empty = w.raw == -INFINITY && w.l == w.l;
+  const float log_l = logf(w.l);
+  // what the reference's rounding added to the sums' logarithm
+  const float residue = fabsf(w.raw) < 1e37f ? fmaf(w.raw, kLog2e, -w.r2) * kLn2 : 0.f;
+  auto log_prob = [&](float x) {
+    return empty || (x == -INFINITY && w.l == w.l) ? -INFINITY : (x - w.raw) - (log_l - residue);
+  };
   if (tid == 0) {
     a.logprob[t] = log_prob(given);
-    if (a.entropy) a.entropy[t] = empty ? 0.f : log_l - r.s / r.l;
-    if (a.rank) a.rank[t] = r.above + 1;
+    if (a.entropy) a.entropy[t] = empty ? 0.f : log_l - kLn2 * (w.s / w.l);
+    if (a.rank) a.rank[t] = w.above + 1;
   }
   auto put = [&](int place, unsigned long long k) {
     a.top_ids[t * a.top + place] = k == 0 ? -1 : 0x7fffffff - static_cast<int>(k & 0xffffffffu);
@@ -362,14 +484,15 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
   if (ranks == 1) {
     if (tid < a.top) put(tid, mine);
   } else {
-    for (int i = tid; i < ranks * a.top; i += kLpThreads) {
-      const unsigned long long k = s_share[i / a.top].top[i % a.top];
+    for (int i = tid; i < ranks * kMaxTop; i += kLpThreads) {
+      const unsigned long long k = s_share[i / kMaxTop].top[i % kMaxTop];
+      if (k == 0) continue;
       int place = 0;
-      for (int j = 0; j < ranks; ++j)
-        for (int p = 0; p < a.top; ++p) {
-          const unsigned long long o = s_share[j].top[p];
-          place += o > k || (o == k && j * a.top + p < i);  // ties only between places that are empty (0)
-        }
+      for (int j = 0; j < ranks; ++j) {
+        const ulonglong2* o = reinterpret_cast<const ulonglong2*>(s_share[j].top);
+#pragma unroll
+        for (int p = 0; p < kMaxTop / 2; ++p) place += (o[p].x > k) + (o[p].y > k);
+      }
       if (place < a.top) put(place, k);
     }
   }
@@ -377,10 +500,10 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
 
 template <typename T>
 cudaError_t launch(const LogprobArgs& a, int num_sms, cudaStream_t stream) {
-  // CTAs per row: enough to fill the GPU with few rows, while a CTA still has
-  // a vector for each of its threads
+  // CTAs per row: as many as run at once, while each still has a vector for
+  // each of its threads
   int ranks = 1;
-  while (ranks < 8 && static_cast<int64_t>(a.rows) * ranks < 4 * num_sms &&
+  while (ranks < 8 && static_cast<int64_t>(a.rows) * 2 * ranks <= kLpPerSm * num_sms &&
          static_cast<int64_t>(a.vocab) >= static_cast<int64_t>(2 * ranks) * kLpThreads * Vec<T>::N)
     ranks *= 2;
   cudaLaunchAttribute attr[1];

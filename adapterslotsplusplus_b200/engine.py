@@ -39,7 +39,14 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
     return code
 
 
+# the raw handle without a Stream object around it (2 us a call less), where
+# this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -55,9 +62,15 @@ def _packed_rows(t: torch.Tensor, what: str) -> torch.Tensor:
     when the strides or the address do not allow them."""
     if not t.is_cuda:
         raise RuntimeError(f"{what} must be a CUDA tensor")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    tokens, heads, dim = t.stride()
+    if dim != 1 or tokens % 8 or heads % 8 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format)
     return t
+
+
+def _empty_rows(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor like t."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 class TokenLogprobs(NamedTuple):
@@ -374,18 +387,21 @@ class WarpPipeEngine:
         keys, kv_heads, k_dim = k.shape
         if k_dim != dim or kv_heads == 0 or heads == 0 or heads % kv_heads:
             raise RuntimeError(f"prompt_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not go together")
-        q, k, v = (_packed_rows(t, "prompt_attention: q/k/v") for t in (q, k, v))
+        q = _packed_rows(q, "prompt_attention: q")
+        k = _packed_rows(k, "prompt_attention: k")
+        v = _packed_rows(v, "prompt_attention: v")
         cu_q = _index(cu_q, "prompt_attention: cu_q", 1)
         cu_k = cu_q if cu_k is None else _index(cu_k, "prompt_attention: cu_k", 1)
-        n = int(cu_q.numel()) - 1
-        if n < 0 or int(cu_k.numel()) != n + 1:
+        n = cu_q.numel() - 1
+        if n < 0 or cu_k.numel() != n + 1:
             raise RuntimeError("prompt_attention: cu_q and cu_k must have one entry more than there are sequences")
-        out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=q.device)
+        out = _empty_rows(q)
         lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
         self._check(self._lib.wp_prompt_attention(
-            self._h, out.data_ptr(), None if lse is None else lse.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cu_q.data_ptr(),
-            cu_k.data_ptr(), n, tokens if max_q is None else int(max_q), tokens, keys, heads, kv_heads, dim,
+            self._h, out.data_ptr(), None if lse is None else lse.data_ptr(), q.data_ptr(), qs[0], qs[1], k.data_ptr(),
+            ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(), n,
+            tokens if max_q is None else int(max_q), tokens, keys, heads, kv_heads, dim,
             dim ** -0.5 if scale is None else float(scale), dt, _stream_ptr(q.device)))
         return (out, lse) if return_lse else out
 
@@ -401,26 +417,29 @@ class WarpPipeEngine:
         code = _lib.WP_DTYPE_F32 if logits.dtype == torch.float32 else _dtype_code(logits, "token_logprobs: logits")
         if tokens.dtype not in (torch.int32, torch.int64):
             raise RuntimeError("token_logprobs: tokens must be int32 or int64")
-        if logits.dim() != 2 or tokens.dim() != 1 or int(tokens.size(0)) != int(logits.size(0)):
+        if logits.dim() != 2 or tokens.dim() != 1 or tokens.numel() != logits.size(0):
             raise RuntimeError("token_logprobs: logits must be [rows, vocab] and tokens [rows]")
-        rows, vocab = int(logits.size(0)), int(logits.size(1))
+        rows, vocab = logits.shape
         top = int(top)
         if top < 0 or top > 32 or top > vocab:
             raise RuntimeError(f"token_logprobs: top must be 0..32 and at most the vocabulary ({vocab}), got {top}")
-        if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
+        ld, step = logits.stride()
+        if step != 1 or (rows > 1 and ld < vocab):
             logits = logits.contiguous()
-        tokens = tokens.contiguous()
+            ld = vocab
+        if not tokens.is_contiguous():
+            tokens = tokens.contiguous()
         dev = logits.device
         f = torch.empty(rows * (2 + top), dtype=torch.float32, device=dev)
         i = torch.empty(rows * (1 + top), dtype=torch.int32, device=dev)
-        res = TokenLogprobs(f[:rows], i[:rows], f[rows:2 * rows], i[rows:].view(rows, top), f[2 * rows:].view(rows, top))
         fp, ip = f.data_ptr(), i.data_ptr()
         self._check(self._lib.wp_token_logprobs(
-            self._h, fp, ip, fp + 4 * rows, ip + 4 * rows, fp + 8 * rows, logits.data_ptr(),
-            max(int(logits.stride(0)), vocab), tokens.data_ptr(),
-            _lib.WP_DTYPE_I64 if tokens.dtype == torch.int64 else _lib.WP_DTYPE_I32, rows, vocab, top, code,
-            _stream_ptr(dev)))
-        return res
+            self._h, fp, ip, fp + 4 * rows, ip + 4 * rows, fp + 8 * rows, logits.data_ptr(), max(ld, vocab),
+            tokens.data_ptr(), _lib.WP_DTYPE_I64 if tokens.dtype == torch.int64 else _lib.WP_DTYPE_I32, rows, vocab, top,
+            code, _stream_ptr(dev)))
+        logprob, entropy, top_logprobs = f.split((rows, rows, rows * top))
+        rank, top_ids = i.split((rows, rows * top))
+        return TokenLogprobs(logprob, rank, entropy, top_ids.view(rows, top), top_logprobs.view(rows, top))
 
     # -- staging slots (engine.py:44-54) -----------------------------------------
     def prefetch_adapter(self, adapter_id) -> int:

@@ -19,12 +19,12 @@ its context back with `read` and runs WarpPipeEngine.prompt_attention on it.
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import _lib
-from .engine import WarpPipeEngine, _DTYPES, _dtype_code, _index, _packed_rows, _stream_ptr
+from .engine import WarpPipeEngine, _DTYPES, _empty_rows, _index, _packed_rows, _stream_ptr
 
 
 class KvCache4:
@@ -56,24 +56,26 @@ class KvCache4:
         self.page_size = int(pages.size(2)) * self.TILE
         self.head_dim = (int(pages.size(3)) - 128) // 16
         self._code = _DTYPES[dtype]
+        self._work_bytes: Dict[Tuple[int, int], int] = {}  # (heads, max_q) -> attention's workspace
 
     def _place(self, table, lens, cu, tokens: int, what: str) -> Tuple:
         table = _index(table, f"{what}: table", 2)
         lens = _index(lens, f"{what}: lens", 1)
-        n = int(lens.numel())
-        if int(table.size(0)) != n:
+        n = lens.numel()
+        if table.size(0) != n:
             raise RuntimeError(f"{what}: table and lens must have one row per sequence")
         if cu is None:
             if tokens != n:
                 raise RuntimeError(f"{what}: without cu every sequence has one token")
         else:
             cu = _index(cu, f"{what}: cu", 1)
-            if int(cu.numel()) != n + 1:
+            if cu.numel() != n + 1:
                 raise RuntimeError(f"{what}: cu must have one entry more than there are sequences")
         return table, lens, cu, n
 
     def _rows(self, t: torch.Tensor, heads: int, what: str) -> torch.Tensor:
-        if t.dim() != 3 or (heads and int(t.size(1)) != heads) or int(t.size(2)) != self.head_dim:
+        shape = t.shape
+        if len(shape) != 3 or (heads and shape[1] != heads) or shape[2] != self.head_dim:
             raise RuntimeError(f"{what} must be [tokens, {heads or 'heads'}, {self.head_dim}]")
         if t.dtype != self.dtype:
             raise RuntimeError(f"{what} must be of the cache's dtype {self.dtype}, got {t.dtype}")
@@ -85,13 +87,14 @@ class KvCache4:
         [sequences] lengths with these tokens included, cu [sequences + 1]
         offsets of each sequence's tokens (None: one each); int32."""
         k, v = self._rows(k, self.kv_heads, "append: k"), self._rows(v, self.kv_heads, "append: v")
-        tokens = int(k.size(0))
-        if int(v.size(0)) != tokens:
+        tokens = k.size(0)
+        if v.size(0) != tokens:
             raise RuntimeError("append: k and v must have the same number of tokens")
         table, lens, cu, n = self._place(table, lens, cu, tokens, "append")
+        ks, vs = k.stride(), v.stride()
         _lib.check(self._lib.wp_kv4_append(
-            self.engine.handle, self.pages.data_ptr(), self.num_pages, self.page_size, k.data_ptr(), k.stride(0),
-            k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), table.data_ptr(), table.size(1), lens.data_ptr(),
+            self.engine.handle, self.pages.data_ptr(), self.num_pages, self.page_size, k.data_ptr(), ks[0], ks[1],
+            v.data_ptr(), vs[0], vs[1], table.data_ptr(), table.size(1), lens.data_ptr(),
             None if cu is None else cu.data_ptr(), n, tokens, self.kv_heads, self.head_dim, self._code,
             _stream_ptr(self.pages.device)), self.engine.handle)
 
@@ -123,20 +126,24 @@ class KvCache4:
         softmax's log denominators [tokens, heads] in fp32 with return_lse. A
         row that sees nothing is 0 (lse -inf)."""
         q = self._rows(q, 0, "attention: q")
-        tokens, heads = int(q.size(0)), int(q.size(1))
+        tokens, heads, _ = q.shape
         if heads == 0 or heads % self.kv_heads:
             raise RuntimeError(f"attention: q has {heads} heads, not a multiple of the cache's {self.kv_heads}")
         table, lens, cu, n = self._place(table, lens, cu, tokens, "attention")
-        h = self.engine.handle
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
-        size = self._lib.wp_kv4_attention_workspace(h, heads, self.kv_heads, self.head_dim, int(max_q), self._code)
+        h, dev, max_q = self.engine.handle, q.device, int(max_q)
+        out = _empty_rows(q)
+        lse = torch.empty(tokens, heads, dtype=torch.float32, device=dev) if return_lse else None
+        size = self._work_bytes.get((heads, max_q))
+        if size is None:
+            size = self._work_bytes[heads, max_q] = max(
+                self._lib.wp_kv4_attention_workspace(h, heads, self.kv_heads, self.head_dim, max_q, self._code), 0)
         # from the caching allocator, so that calls on several streams never share it
-        work = torch.empty(max(size, 0), dtype=torch.uint8, device=q.device)
+        work = torch.empty(size, dtype=torch.uint8, device=dev)
+        qs = q.stride()
         _lib.check(self._lib.wp_kv4_attention(
-            h, out.data_ptr(), None if lse is None else lse.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
-            self.pages.data_ptr(), self.num_pages, self.page_size, table.data_ptr(), table.size(1), lens.data_ptr(),
-            None if cu is None else cu.data_ptr(), n, int(max_q), tokens, heads, self.kv_heads, self.head_dim,
+            h, out.data_ptr(), None if lse is None else lse.data_ptr(), q.data_ptr(), qs[0], qs[1], self.pages.data_ptr(),
+            self.num_pages, self.page_size, table.data_ptr(), table.size(1), lens.data_ptr(),
+            None if cu is None else cu.data_ptr(), n, max_q, tokens, heads, self.kv_heads, self.head_dim,
             1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), self._code, work.data_ptr(), size,
-            _stream_ptr(q.device)), h)
+            _stream_ptr(dev)), h)
         return (out, lse) if return_lse else out
