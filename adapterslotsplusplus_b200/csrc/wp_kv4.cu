@@ -45,6 +45,13 @@ __device__ __forceinline__ float to_float(uint32_t bits16) {
   return Elem<T>::to_f(*reinterpret_cast<const T*>(&u));
 }
 
+// x / group for the packed rows of a kv head (x * group < 2^32), without a division.
+struct GroupDiv {
+  uint32_t group, magic;
+  __device__ __forceinline__ explicit GroupDiv(int g) : group(g), magic(g == 1 ? 0 : 0xffffffffu / g + 1) {}
+  __device__ __forceinline__ int div(int x) const { return group == 1 ? x : static_cast<int>(__umulhi(x, magic)); }
+};
+
 struct Seq {
   int first;  // packed row of its first token
   int n;  // tokens of this call
@@ -88,21 +95,36 @@ __device__ __forceinline__ uint8_t* tile_ptr(const Kv4Args& a, int b, int h, int
 
 // ---- append and read ----------------------------------------------------------
 //
-// One CTA per (sequence, head) and tile of 16 tokens; each warp takes single
-// tokens of K or V. Bound by memory: 4 D bytes of K and V in, D + 8 out
-// (append), or the reverse. A tile whose 16 tokens are all new leaves shared
-// memory in 16-byte stores; in a tile that is shared with older tokens only
-// the new tokens' bytes are written (a token owns whole bytes of both blocks).
+// One CTA per (sequence, head) and tile of 16 tokens. A lane has 16 dimensions
+// of one token of K or V: 32 contiguous bytes in 16 bits, 8 bytes of codes (of
+// V, whole bytes: dimensions g and g + 8 share one), and the minimum and
+// maximum of a row need log2(D / 16) exchanges. Bound by memory: 4 D bytes of K
+// and V in, D + 8 out (append), or the reverse. A tile whose 16 tokens are all
+// new leaves shared memory in 16-byte stores; in a tile that is shared with
+// older tokens only the new tokens' bytes are written (a token owns whole bytes
+// of both blocks).
 
 constexpr int kMoveThreads = 128;
+
+// The nearest code to d / step, as rint of the correctly rounded quotient: the
+// product with the reciprocal (inv) is within 2^-17 of it and decides unless it
+// is about half-way between two codes.
+__device__ __forceinline__ uint32_t code_of(float d, float step, float inv) {
+  float r = d * inv, k = rintf(r);
+  if (!(fabsf(r - k) <= 0.4999f)) k = step > 0.f ? rintf(__fdiv_rn(d, step)) : 0.f;
+  return static_cast<uint32_t>(fminf(fmaxf(k, 0.f), 15.f));
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Kv4Args a, int per_seq) {
   constexpr int TB = kv4_tile_bytes(D);
-  constexpr int PER = D / 32;  // dimensions per lane
+  constexpr int PER = D / 16;  // lanes per row
+  constexpr int RW = 32 / PER;  // rows per warp; even warps take K, odd ones V
+  constexpr int N = kKv4Tile / (kMoveThreads / 64 * RW);
   __shared__ __align__(16) uint8_t tile[TB];
   const int b = blockIdx.x / per_seq, h = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, part = threadIdx.x % PER, is_v = warp & 1;
+  const int tok0 = (warp >> 1) * RW + (threadIdx.x & 31) / PER;  // tokens tok0 + kMoveThreads / 64 * RW * n
   const Seq s = load_seq(a, b);
   if (s.n > s.len) {  // more new tokens than the sequence has
     if (threadIdx.x == 0 && a.err) atomicOr(a.err, kErrBadSegment);
@@ -114,55 +136,58 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Kv4Args a, int
     const int lo = max(start - t * kKv4Tile, 0), hi = min(s.len - t * kKv4Tile, kKv4Tile);
     uint8_t* dst = tile_ptr(a, b, h, t, TB);
     if (dst == nullptr) continue;  // the same for the whole CTA
-    for (int u = 2 * lo + warp; u < 2 * hi; u += kMoveThreads / 32) {
-      const int tok = u >> 1, is_v = u & 1;
-      const int64_t row = s.first + (t * kKv4Tile + tok - start);
-      const T* src = static_cast<const T*>(is_v ? a.v : a.k) + row * (is_v ? a.v_ts : a.k_ts) +
-                     static_cast<int64_t>(h) * (is_v ? a.v_hs : a.k_hs) + lane * PER;
-      float x[PER];
-      if constexpr (PER == 4) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
-        const float2 p = Elem<T>::unpack2(w.x), q = Elem<T>::unpack2(w.y);
-        x[0] = p.x, x[1] = p.y, x[2] = q.x, x[3] = q.y;
+    uint4 w[N][2];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int tok = tok0 + kMoveThreads / 64 * RW * n;
+      if (tok >= lo && tok < hi) {
+        const int64_t row = s.first + (t * kKv4Tile + tok - start);
+        const T* src = static_cast<const T*>(is_v ? a.v : a.k) + row * (is_v ? a.v_ts : a.k_ts) +
+                       static_cast<int64_t>(h) * (is_v ? a.v_hs : a.k_hs) + part * 16;
+        w[n][0] = __ldg(reinterpret_cast<const uint4*>(src));
+        w[n][1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
       } else {
-        const float2 p = Elem<T>::unpack2(__ldg(reinterpret_cast<const uint32_t*>(src)));
-        x[0] = p.x, x[1] = p.y;
+        w[n][0] = w[n][1] = make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int tok = tok0 + kMoveThreads / 64 * RW * n;
+      if (__all_sync(~0u, tok < lo || tok >= hi)) continue;
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t u[4] = {w[n][i].x, w[n][i].y, w[n][i].z, w[n][i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = Elem<T>::unpack2(u[j]);
+          x[8 * i + 2 * j] = f.x;
+          x[8 * i + 2 * j + 1] = f.y;
+        }
       }
       float mn = x[0], mx = x[0];
 #pragma unroll
-      for (int i = 1; i < PER; ++i) mn = fminf(mn, x[i]), mx = fmaxf(mx, x[i]);
+      for (int i = 1; i < 16; ++i) mn = fminf(mn, x[i]), mx = fmaxf(mx, x[i]);
 #pragma unroll
-      for (int o = 16; o; o >>= 1) {
+      for (int o = PER / 2; o; o >>= 1) {
         mn = fminf(mn, __shfl_xor_sync(~0u, mn, o));
         mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
       }
       const uint32_t pair = Elem<T>::pack2(__fmul_rn(__fsub_rn(mx, mn), 1.0f / 15.0f), mn);
-      const float step = Elem<T>::unpack2(pair).x;
-      uint32_t code = 0;  // one nibble per dimension
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const float r = step > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[i], mn), step)) : 0.f;
-        code |= static_cast<uint32_t>(fminf(fmaxf(r, 0.f), 15.f)) << (4 * i);
-      }
+      const float step = Elem<T>::unpack2(pair).x, inv = __frcp_rn(step);
+      if (tok < lo || tok >= hi) continue;
       if (!is_v) {
-        if constexpr (PER == 4)
-          *reinterpret_cast<uint16_t*>(tile + tok * (D / 2) + lane * 2) = static_cast<uint16_t>(code);
-        else
-          tile[tok * (D / 2) + lane] = static_cast<uint8_t>(code);
-      } else {
-        // dimensions 16 m + g and + 8 share a byte: the lane 8 dimensions on has the upper half
-        const uint32_t up = __shfl_down_sync(~0u, code, 8 / PER);
-        const int d0 = lane * PER;
-        if ((d0 & 15) < 8) {
+        uint32_t c[2] = {0, 0};  // one nibble per dimension
 #pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const int d = d0 + i;
-            tile[8 * D + v_byte(d >> 6, (d >> 4) & 3, d & 7, tok)] =
-                static_cast<uint8_t>(((code >> (4 * i)) & 15u) | (((up >> (4 * i)) & 15u) << 4));
-          }
-        }
+        for (int i = 0; i < 16; ++i) c[i >> 3] |= code_of(__fsub_rn(x[i], mn), step, inv) << (4 * (i & 7));
+        *reinterpret_cast<uint2*>(tile + tok * (D / 2) + part * 8) = make_uint2(c[0], c[1]);
+      } else {
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+          tile[8 * D + v_byte(part >> 2, part & 3, g, tok)] = static_cast<uint8_t>(
+              code_of(__fsub_rn(x[g], mn), step, inv) | (code_of(__fsub_rn(x[g + 8], mn), step, inv) << 4));
       }
-      if (lane == 0) *reinterpret_cast<uint32_t*>(tile + 16 * D + is_v * 64 + tok * 4) = pair;
+      if (part == 0) *reinterpret_cast<uint32_t*>(tile + 16 * D + is_v * 64 + tok * 4) = pair;
     }
     __syncthreads();
     if (lo == 0 && hi == kKv4Tile) {
@@ -170,11 +195,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Kv4Args a, int
         reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(tile)[i];
     } else {
       const int nt = hi - lo;
-      for (int i = threadIdx.x; i < nt * (D / 8); i += kMoveThreads) {  // K rows and scales, 4 bytes each
+      for (int i = threadIdx.x; i < nt * (D / 8); i += kMoveThreads) {  // K rows, 4 bytes each
         const int o = lo * (D / 2) + i * 4;
         *reinterpret_cast<uint32_t*>(dst + o) = *reinterpret_cast<const uint32_t*>(tile + o);
       }
-      for (int i = threadIdx.x; i < nt * 2; i += kMoveThreads) {
+      for (int i = threadIdx.x; i < nt * 2; i += kMoveThreads) {  // scales
         const int o = 16 * D + (i & 1) * 64 + (lo + (i >> 1)) * 4;
         *reinterpret_cast<uint32_t*>(dst + o) = *reinterpret_cast<const uint32_t*>(tile + o);
       }
@@ -190,6 +215,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Kv4Args a, int
 template <typename T, int D>
 __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Kv4Args a, int per_seq) {
   constexpr int TB = kv4_tile_bytes(D);
+  constexpr int PER = D / 16;
   __shared__ __align__(16) uint8_t tile[TB];
   const int b = blockIdx.x / per_seq, h = blockIdx.y;
   const Seq s = load_seq(a, b);
@@ -206,27 +232,33 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Kv4Args a, int p
     for (int i = threadIdx.x; i < TB / 16; i += kMoveThreads)
       reinterpret_cast<uint4*>(tile)[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
     __syncthreads();
-    // 8 dimensions of one token of K or V per thread
-    for (int i = threadIdx.x; i < (hi - lo) * (D / 4); i += kMoveThreads) {
-      const int d8 = i % (D / 8), is_v = (i / (D / 8)) & 1, tok = lo + i / (D / 4);
-      uint32_t codes = 0;  // one nibble per dimension
+    // 16 dimensions of one token of K or V per thread and pass
+    for (int i = threadIdx.x; i < 2 * kKv4Tile * PER; i += kMoveThreads) {
+      const int part = i % PER, tok = (i / PER) & 15, is_v = i / (PER * kKv4Tile);
+      if (tok < lo || tok >= hi) continue;
+      const float2 sz = Elem<T>::unpack2(*reinterpret_cast<const uint32_t*>(tile + 16 * D + is_v * 64 + tok * 4));
+      auto value = [&](uint32_t c) { return fmaf(sz.x, static_cast<float>(c & 15u), sz.y); };
+      uint32_t w[8];  // the 16 values, in pairs
       if (!is_v) {
-        codes = *reinterpret_cast<const uint32_t*>(tile + tok * (D / 2) + d8 * 4);
+        const uint2 c = *reinterpret_cast<const uint2*>(tile + tok * (D / 2) + part * 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t u = (j < 4 ? c.x : c.y) >> (8 * (j & 3));
+          w[j] = Elem<T>::pack2(value(u), value(u >> 4));
+        }
       } else {
-        const int hh = d8 >> 3, m = (d8 >> 1) & 3, sh = (d8 & 1) * 4;
+        const uint8_t* v = tile + 8 * D + v_byte(part >> 2, part & 3, 0, tok);
 #pragma unroll
-        for (int g = 0; g < 8; ++g) codes |= static_cast<uint32_t>((tile[8 * D + v_byte(hh, m, g, tok)] >> sh) & 15) << (4 * g);
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t u0 = v[128 * j], u1 = v[128 * j + 64];  // dimensions 2j, 2j + 1 (and + 8)
+          w[j] = Elem<T>::pack2(value(u0), value(u1));
+          w[4 + j] = Elem<T>::pack2(value(u0 >> 4), value(u1 >> 4));
+        }
       }
-      const uint32_t pair = *reinterpret_cast<const uint32_t*>(tile + 16 * D + is_v * 64 + tok * 4);
-      const float2 sz = Elem<T>::unpack2(pair);
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = Elem<T>::pack2(fmaf(sz.x, static_cast<float>((codes >> (8 * j)) & 15u), sz.y),
-                              fmaf(sz.x, static_cast<float>((codes >> (8 * j + 4)) & 15u), sz.y));
       const int64_t row = s.first + (t * kKv4Tile + tok - start);
-      T* dst = static_cast<T*>(is_v ? a.v : a.k) + (row * a.kv_heads + h) * D + d8 * 8;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(is_v ? a.v : a.k) + (row * a.kv_heads + h) * D + part * 16);
+      dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
     __syncthreads();
   }
@@ -254,17 +286,21 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Kv4Args a, int p
 // which kv4_combine_kernel adds in order (no atomics: results do not depend on
 // timing).
 
-constexpr int kAttnWarps = 8;
-constexpr int kAttnThreads = kAttnWarps * 32;
-
+// Twelve warps of 168 registers hide the latencies of the short dependent steps
+// (softmax, scales) that eight did not (two per scheduler issued in 47% of the
+// cycles); 16 query rows need 255 registers and stay at eight.
 template <int D, int NT>
 struct AttnCfg {
+  static constexpr int WARPS = NT == 1 ? 12 : 8;
+  static constexpr int THREADS = WARPS * 32;
   static constexpr int TB = kv4_tile_bytes(D);
   static constexpr int TILES = kKv4Chunk / kKv4Tile;  // tiles of one chunk
   static constexpr int STAGE = TILES * TB;
-  static constexpr int S = 3;  // stages of a warp's ring
-  static constexpr int BARS = 1024;  // mbarriers and the block's prefix sums (see the kernel)
-  static constexpr int SMEM = 2 * BARS + kAttnWarps * S * STAGE;
+  static constexpr int S = (NT == 1 ? 2 : 3) * (D == 64 ? 2 : 1);  // stages of a warp's ring
+  static constexpr int BARS = 1024;  // mbarriers
+  static constexpr int HEAD = BARS + THREADS * 4;  // and the block's prefix sums (see the kernel)
+  static constexpr int SMEM = HEAD + WARPS * S * STAGE;
+  static_assert(SMEM <= 232448 && HEAD % 16 == 0, "shared memory budget");
   static constexpr int ROWS = 8 * NT;
 };
 
@@ -298,8 +334,9 @@ struct Cursor {
 __device__ __forceinline__ long long range_start(long long total, int w, int n) { return total * w / n; }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv4Args a) {
+__global__ void __launch_bounds__(AttnCfg<D, NT>::THREADS, 1) kv4_attention_kernel(const Kv4Args a) {
   using C = AttnCfg<D, NT>;
+  constexpr int kAttnWarps = C::WARPS, kAttnThreads = C::THREADS;
   using E = Elem<T>;
   constexpr int MT = D / 16;  // 16-dimension tiles of the output
   constexpr int KW = D / 32;  // code words (8 dimensions) of a lane's K row; two k16 steps each
@@ -308,6 +345,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
   int* s_sum = reinterpret_cast<int*>(smem + C::BARS);  // chunks of the sequences of thread i's slice, then their prefix
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int group = a.heads / a.kv_heads;
+  const GroupDiv by(group);
 
   // ---- the call's chunks: each thread counts a contiguous slice of sequences
   const int slice = (a.num_seqs + kAttnThreads - 1) / kAttnThreads;
@@ -371,18 +409,38 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
   }
 
   // ---- the ring
-  uint8_t* ring = smem + 2 * C::BARS + warp * C::S * C::STAGE;
+  uint8_t* ring = smem + C::HEAD + warp * C::S * C::STAGE;
   uint64_t* bar = bars + warp * C::S;
   const int count = static_cast<int>(w1 - w0);
   Cursor pro = con;
   int issued = 0;
   const uint8_t* src = nullptr;  // lane i < TILES: tile i of the next chunk to issue
-  auto find = [&] {
-    src = nullptr;
+  int slot = 0, off = 0;  // its page slot and the tile's place in the page
+  auto find = [&](bool jump) {
     const int tile = pro.t * C::TILES + lane;
+    if (jump) {
+      slot = tile / a.page_tiles;
+      off = tile - slot * a.page_tiles;
+    } else {
+      for (off += C::TILES; off >= a.page_tiles; off -= a.page_tiles) ++slot;
+    }
+    src = nullptr;
     if (lane < C::TILES && tile * kKv4Tile < pro.s.len) {
-      src = tile_ptr(a, pro.b, pro.h, tile, C::TB);
-      if (src == nullptr) src = a.pages;  // bad page: any readable tile
+      const int page = __ldg(a.table + static_cast<int64_t>(pro.b) * a.table_ld + slot);
+      src = a.pages;  // a bad page number: any readable tile, and the error bit
+      if (page >= 0 && page < a.num_pages)
+        src += ((static_cast<int64_t>(page) * a.kv_heads + pro.h) * a.page_tiles + off) * C::TB;
+      else if (a.err)
+        atomicOr(a.err, kErrBadSegment);
+    }
+    if (jump && lane < C::ROWS) {  // the segment's query rows will be wanted soon
+      const int r = pro.rb * C::ROWS + lane;
+      if (r < pro.s.n * group) {
+        const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(pro.s.first + by.div(r)) * a.q_ts +
+                      static_cast<int64_t>(pro.h * group + r - by.div(r) * group) * a.q_hs;
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(qp));
+        if (D == 128) asm volatile("prefetch.global.L1 [%0];" ::"l"(qp + 64));
+      }
     }
   };
   auto issue = [&] {  // src was found one chunk earlier, so its page number has arrived
@@ -393,10 +451,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
     if (src != nullptr) bulk_g2s(ring + st * C::STAGE + lane * C::TB, src, C::TB, &bar[st]);
     if (++issued < count) {
       pro.next(a, group, C::ROWS);
-      find();
+      find(pro.t == 0);
     }
   };
-  find();
+  find(true);
   for (int i = 0; i < C::S - 1 && issued < count; ++i) issue();
 
   // ---- the range, segment by segment
@@ -426,8 +484,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
         uint4 w[KW];
         float mx = 0.f, sum = 0.f;
         const bool row = r < con.s.n * group;
-        const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(con.s.first + r / group) * a.q_ts +
-                      static_cast<int64_t>(con.h * group + r % group) * a.q_hs + c * (D / 4);
+        const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(con.s.first + by.div(r)) * a.q_ts +
+                      static_cast<int64_t>(con.h * group + r - by.div(r) * group) * a.q_hs + c * (D / 4);
 #pragma unroll
         for (int i = 0; i < KW; ++i) {
           w[i] = row ? __ldg(reinterpret_cast<const uint4*>(qp) + i) : make_uint4(0, 0, 0, 0);
@@ -464,7 +522,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
           qa[nt][j] = __shfl_sync(~0u, sum, (2 * c + j) * 4);
           qb[nt][j] = __shfl_sync(~0u, up, (2 * c + j) * 4);
           const int rr = con.rb * C::ROWS + nt * 8 + 2 * c + j;
-          lim[nt][j] = min(con.s.len - (con.s.n - 1) + rr / group, con.s.len);
+          lim[nt][j] = min(con.s.len - (con.s.n - 1) + by.div(rr), con.s.len);
           m[nt][j] = -INFINITY;
           l[nt][j] = pz[nt][j] = wtop[nt][j] = 0.f;
           wexp[nt][j] = 40u << 23;
@@ -493,6 +551,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
       for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
       for (int ti = 0; ti < C::TILES; ++ti) {
+        if (ti * kKv4Tile >= left) {  // no token of the tile is left
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[ti][nt][j] = -INFINITY;
+          vs[ti][0] = vs[ti][1] = make_float2(0.f, 0.f);
+          continue;
+        }
         const uint8_t* tp = sp + ti * C::TB;
         uint32_t k0[KW], k1[KW];
         if constexpr (KW == 4) {
@@ -505,10 +571,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
           const uint2 v = *reinterpret_cast<const uint2*>(tp + 256 + g * 32 + c * 8);
           k0[0] = u.x, k0[1] = u.y, k1[0] = v.x, k1[1] = v.y;
         }
+        float s2[NT][4];  // a second accumulator: half as long a chain of dependent products
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[ti][nt][j] = 0.f;
+          for (int j = 0; j < 4; ++j) s[ti][nt][j] = s2[nt][j] = 0.f;
 #pragma unroll
         for (int i = 0; i < KW; ++i) {
           const uint32_t x0 = k0[i] >> 8, x1 = k1[i] >> 8;
@@ -517,7 +584,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma_k16<__half>(s[ti][nt], fa, qf[nt][i][0], qf[nt][i][1]);
-            mma_k16<__half>(s[ti][nt], fb, qf[nt][i][2], qf[nt][i][3]);
+            mma_k16<__half>(s2[nt], fb, qf[nt][i][2], qf[nt][i][3]);
           }
         }
         const float2 kz0 = E::unpack2(*reinterpret_cast<const uint32_t*>(tp + 16 * D + g * 4));
@@ -530,8 +597,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            s[ti][nt][j] = fmaf(s[ti][nt][j] * kz0.x, qb[nt][j], kz0.y * qa[nt][j]);
-            s[ti][nt][2 + j] = fmaf(s[ti][nt][2 + j] * kz1.x, qb[nt][j], kz1.y * qa[nt][j]);
+            s[ti][nt][j] = fmaf((s[ti][nt][j] + s2[nt][j]) * kz0.x, qb[nt][j], kz0.y * qa[nt][j]);
+            s[ti][nt][2 + j] = fmaf((s[ti][nt][2 + j] + s2[nt][2 + j]) * kz1.x, qb[nt][j], kz1.y * qa[nt][j]);
           }
         if (masked) {
           // what a row must not see counts as minus infinity whatever the
@@ -572,7 +639,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
           wtop[nt][j] *= f[nt][j];
         }
 #pragma unroll
-        for (int ti = 0; ti < C::TILES; ++ti)
+        for (int ti = 0; ti < C::TILES; ++ti) {
+          if (ti * kKv4Tile >= left) break;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float p = ex2(s[ti][nt][j] - base[j & 1]);
@@ -583,6 +651,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
             s[ti][nt][j] = w;
             big[j & 1] = fmaxf(big[j & 1], w);
           }
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -617,6 +686,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
         for (int j = 0; j < 2; ++j) down[nt][j] = __uint_as_float(((254u + 14u) << 23) - wexp[nt][j]);  // 2^(14 - e)
 #pragma unroll
       for (int ti = 0; ti < C::TILES; ++ti) {
+        if (ti * kKv4Tile >= left) break;
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -677,8 +747,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
 #pragma unroll
           for (int j = 0; j < 2; ++j) inv[j] = l[nt][j] == 0.f ? 0.f : 1.f / l[nt][j];
           const int r = con.rb * C::ROWS + nt * 8 + g;  // after the transpose this lane has row g, dimensions 2c, 2c + 1
-          const int64_t tok = con.s.first + r / group;
-          T* op = static_cast<T*>(a.out) + (tok * a.heads + con.h * group + r % group) * D + 2 * c;
+          const int64_t tok = con.s.first + by.div(r);
+          T* op = static_cast<T*>(a.out) + (tok * a.heads + con.h * group + r - by.div(r) * group) * D + 2 * c;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -691,7 +761,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
             const int rr = con.rb * C::ROWS + nt * 8 + 2 * c + g;
             const float lj = g ? l[nt][1] : l[nt][0], mj = g ? m[nt][1] : m[nt][0];
             if (rr < rows)
-              a.lse[(con.s.first + rr / group) * static_cast<int64_t>(a.heads) + con.h * group + rr % group] =
+              a.lse[(con.s.first + by.div(rr)) * static_cast<int64_t>(a.heads) + con.h * group + rr - by.div(rr) * group] =
                   lj == 0.f ? -INFINITY : (mj + __log2f(lj)) * kLn2;
           }
         }
@@ -728,8 +798,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) kv4_attention_kernel(const Kv
 // Adds the partial rows of segments that several warps shared, in warp order.
 // A warp takes a quarter of one row's dimensions; its four lane groups take
 // every fourth part.
+constexpr int kJoinWarps = 8;
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads) kv4_combine_kernel(const Kv4Args a, int warps) {
+__global__ void __launch_bounds__(kJoinWarps * 32) kv4_combine_kernel(const Kv4Args a, int warps) {
   using C = AttnCfg<D, NT>;
   constexpr int Q = D / 4;  // dimensions per unit
   constexpr int LANES = Q / 4;  // lanes per part: float4 each
@@ -740,9 +812,9 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_combine_kernel(const Kv4Args
   // A warp has one (row, quarter) and every ngrp-th first warp of a segment;
   // most of those have no shared segment, so their descriptors are read 32 at
   // a time.
-  const int gw = blockIdx.x * kAttnWarps + (threadIdx.x >> 5);
+  const int gw = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
   const int quarter = gw & 3, row = (gw >> 2) % C::ROWS, grp = gw / (4 * C::ROWS);
-  const int ngrp = gridDim.x * kAttnWarps / (4 * C::ROWS);
+  const int ngrp = gridDim.x * kJoinWarps / (4 * C::ROWS);
   for (int base = grp; base < warps; base += ngrp * 32) {
     const int4 mine = base + lane * ngrp < warps ? __ldcg(a.part_desc + 2 * (base + lane * ngrp)) : make_int4(0, 0, 0, 0);
     for (unsigned todo = __ballot_sync(~0u, mine.x != 0 && row < mine.w); todo; todo &= todo - 1) {
@@ -806,7 +878,7 @@ struct Attn {
     n = 0;
     if (cudaFuncSetAttribute(kv4_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
             cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv4_attention_kernel<T, D, NT>, kAttnThreads, C::SMEM) !=
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv4_attention_kernel<T, D, NT>, C::THREADS, C::SMEM) !=
             cudaSuccess)
       return 0;
     known.store(n);
@@ -814,18 +886,18 @@ struct Attn {
   }
   static int64_t workspace(int num_sms) {
     using C = AttnCfg<D, NT>;
-    const int64_t warps = static_cast<int64_t>(per_sm()) * num_sms * kAttnWarps;
+    const int64_t warps = static_cast<int64_t>(per_sm()) * num_sms * C::WARPS;
     return warps * (2 * C::ROWS * (D * 4 + 8) + 32);
   }
   static cudaError_t launch(Kv4Args a, void* ws, int num_sms, cudaStream_t stream) {
     using C = AttnCfg<D, NT>;
     const int grid = per_sm() * num_sms;
     if (grid == 0) return cudaErrorInvalidConfiguration;
-    const int64_t warps = static_cast<int64_t>(grid) * kAttnWarps;
+    const int64_t warps = static_cast<int64_t>(grid) * C::WARPS;
     a.part_desc = static_cast<int4*>(ws);
     a.part = reinterpret_cast<float*>(a.part_desc + 2 * warps);
     a.part_ml = reinterpret_cast<float2*>(a.part + 2 * warps * C::ROWS * D);
-    kv4_attention_kernel<T, D, NT><<<grid, kAttnThreads, C::SMEM, stream>>>(a);
+    kv4_attention_kernel<T, D, NT><<<grid, C::THREADS, C::SMEM, stream>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
@@ -833,7 +905,7 @@ struct Attn {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(num_sms * 8);  // 8 warps each: every shared row's quarter finds a warp of its own
-    cfg.blockDim = dim3(kAttnThreads);
+    cfg.blockDim = dim3(kJoinWarps * 32);
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
