@@ -465,9 +465,9 @@ __global__ void __launch_bounds__(AttnCfg<D, NT>::THREADS, 1) kv4_attention_kern
   float sumw[NT][4];  // sum of the rounded weights of rows (2c, 2c + 1), times 2^10 of acc's unit ([2], [3] are copies)
   float m[NT][2], l[NT][2], pz[NT][2];
   // p * scaleV enters the tensor core in fp16, rounded once, as p * scaleV /
-  // 2^e * 2^14 with 2^e above the row's largest such weight: at most 2^14, and
-  // a normal number down to 2^-28 of the largest
-  float wtop[NT][2];  // the largest weight so far, relative to the present m
+  // 2^e * 2^14 with 2^(e + 1) above the row's largest such weight: at most
+  // 2^15, and a normal number down to 2^-28 of the largest
+  float wtop[NT][2];  // a bound of the weights so far, relative to the present m
   uint32_t wexp[NT][2];  // biased exponent of 2^e, in place
   bool ok = true;
   long long seg0 = 0;  // chunk index of the segment's first chunk
@@ -619,24 +619,42 @@ __global__ void __launch_bounds__(AttnCfg<D, NT>::THREADS, 1) kv4_attention_kern
 #pragma unroll
           for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(top[nt][j], fmaxf(s[ti][nt][j], s[ti][nt][2 + j]));
       }
-      // ---- weights: p = 2^(s - m), s[][][] becomes p * scaleV
-      bool move = false;
+      // ---- the running maximum. It is only a reference, and raised when a
+      // row's grows by more than 8 (log2 units): no exchange between lanes, and
+      // no rescaling, in nearly all chunks.
+      bool grew = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) grew |= top[nt][j] > m[nt][j] + 8.f;
+      grew = __any_sync(~0u, grew);
       float f[NT][2];
 #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) f[nt][0] = f[nt][1] = 1.f;
+      if (grew) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(~0u, top[nt][j], o));
+            const float mn = fmaxf(m[nt][j], top[nt][j]);
+            f[nt][j] = m[nt][j] == -INFINITY ? 0.f : ex2(m[nt][j] - mn);
+            m[nt][j] = mn;
+            l[nt][j] *= f[nt][j];
+            pz[nt][j] *= f[nt][j];
+          }
+      }
+      // ---- weights: p = 2^(s - m), s[][][] becomes p * scaleV
+      bool move = grew;
+      float big[NT][2];
+#pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float base[2], big[2] = {0.f, 0.f};
+        float base[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int o = 4; o <= 16; o <<= 1) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(~0u, top[nt][j], o));
-          const float mn = fmaxf(m[nt][j], top[nt][j]);
-          base[j] = mn == -INFINITY ? 0.f : mn;
-          f[nt][j] = ex2(m[nt][j] - base[j]);  // 0 where nothing was seen before
-          move |= mn > m[nt][j];
-          m[nt][j] = mn;
-          l[nt][j] *= f[nt][j];
-          pz[nt][j] *= f[nt][j];
-          wtop[nt][j] *= f[nt][j];
+          base[j] = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+          big[nt][j] = 0.f;
         }
 #pragma unroll
         for (int ti = 0; ti < C::TILES; ++ti) {
@@ -644,32 +662,34 @@ __global__ void __launch_bounds__(AttnCfg<D, NT>::THREADS, 1) kv4_attention_kern
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float p = ex2(s[ti][nt][j] - base[j & 1]);
-            float w = p * vs[ti][j >> 1].x, z = p * vs[ti][j >> 1].y;
-            if (masked && s[ti][nt][j] == -INFINITY) w = z = 0.f;  // 0 * infinity: an unseen token adds nothing
+            float w = p * vs[ti][j >> 1].x;
+            if (masked && s[ti][nt][j] == -INFINITY) {  // 0 * infinity: an unseen token adds nothing
+              w = 0.f;
+            } else {
+              pz[nt][j & 1] = fmaf(p, vs[ti][j >> 1].y, pz[nt][j & 1]);
+            }
             l[nt][j & 1] += p;
-            pz[nt][j & 1] += z;
             s[ti][nt][j] = w;
-            big[j & 1] = fmaxf(big[j & 1], w);
+            big[nt][j & 1] = fmaxf(big[nt][j & 1], w);
           }
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int o = 4; o <= 16; o <<= 1) big[j] = fmaxf(big[j], __shfl_xor_sync(~0u, big[j], o));
-          move |= big[j] > __uint_as_float(wexp[nt][j]);
-          wtop[nt][j] = fmaxf(wtop[nt][j], big[j]);
-        }
+        for (int j = 0; j < 2; ++j) move |= big[nt][j] > 2.f * __uint_as_float(wexp[nt][j]);
       }
       if (__any_sync(~0u, move)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) big[nt][j] = fmaxf(big[nt][j], __shfl_xor_sync(~0u, big[nt][j], o));
+            wtop[nt][j] = fmaxf(wtop[nt][j] * f[nt][j], big[nt][j]);
             const uint32_t e = min(max((__float_as_uint(wtop[nt][j]) & 0x7f800000u) + 0x00800000u, 40u << 23), 254u << 23);
             const int d = static_cast<int>(wexp[nt][j] >> 23) - static_cast<int>(e >> 23);  // 2^(old - new), in two factors
             const float up = __uint_as_float(static_cast<uint32_t>(127 + d / 2) << 23);
             const float r = f[nt][j] * up * __uint_as_float(static_cast<uint32_t>(127 + d - d / 2) << 23);
             wexp[nt][j] = e;
+            wtop[nt][j] = __uint_as_float(e - 1);  // just below 2^e: what the weights so far stay under
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               acc[mt][nt][j] *= r;
