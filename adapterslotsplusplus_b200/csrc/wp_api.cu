@@ -2067,6 +2067,7 @@ int wp_kv4_append(wp_handle* h, void* pages, int32_t num_pages, int32_t page_siz
   a.v_ts = v_ts;
   a.v_hs = v_hs;
   a.err = h->d_err;
+  a.pdl = h->cfg.use_pdl;
   if (page_size % wp::kKv4Tile) return fail(h, WP_ERR_INVALID, "kv4_append: page_size must be a multiple of 16");
   if (int rc = check_seqs(h, "kv4_append", a, head_dim, dtype)) return rc;
   if (num_seqs == 0 || tokens == 0) return WP_OK;
@@ -2097,6 +2098,7 @@ int wp_kv4_read(wp_handle* h, void* k, void* v, const void* pages, int32_t num_p
   a.k = k;
   a.v = v;
   a.err = h->d_err;
+  a.pdl = h->cfg.use_pdl;
   if (page_size % wp::kKv4Tile) return fail(h, WP_ERR_INVALID, "kv4_read: page_size must be a multiple of 16");
   if (int rc = check_seqs(h, "kv4_read", a, head_dim, dtype)) return rc;
   if (num_seqs == 0 || tokens == 0) return WP_OK;
@@ -2140,6 +2142,7 @@ int wp_kv4_attention(wp_handle* h, void* out, float* lse, const void* q, int64_t
   a.out = out;
   a.lse = lse;
   a.err = h->d_err;
+  a.pdl = h->cfg.use_pdl;
   if (page_size % wp::kKv4Tile) return fail(h, WP_ERR_INVALID, "kv4_attention: page_size must be a multiple of 16");
   if (int rc = check_seqs(h, "kv4_attention", a, head_dim, dtype)) return rc;
   if (heads < 1 || heads % kv_heads)
@@ -2189,6 +2192,7 @@ int wp_token_logprobs(wp_handle* h, float* logprob, int32_t* rank, float* entrop
   a.entropy = entropy;
   a.top_ids = top_ids;
   a.top_logprobs = top_logprobs;
+  a.pdl = h->cfg.use_pdl;
   DeviceGuard dg(h->device);
   cudaError_t e = wp::launch_token_logprobs(dtype, a, h->num_sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(h, WP_ERR_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
@@ -2236,6 +2240,7 @@ int wp_prompt_attention(wp_handle* h, void* out, float* lse, const void* q, int6
   a.max_q = std::min(std::max(max_q, 1), q_tokens);
   a.scale = scale;
   a.err = h->d_err;
+  a.pdl = h->cfg.use_pdl;
   DeviceGuard dg(h->device);
   cudaError_t e = wp::launch_prompt_attention(dtype, a, h->num_sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(h, WP_ERR_CUDA, "prompt_attention launch: %s", cudaGetErrorString(e));

@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(NW * 32) prompt_small_kernel(const __grid_cons
   const uint32_t ring = smem_u32(smem), qs = ring + 4 * C::TILE + warp * 16 * LD;
   const int chunks = a.dim / 8;  // 16-byte pieces of a row; dimensions past dim are zero
 
+  pdl_wait_prior();
   int b = blockIdx.z, rb = blockIdx.x;
   PromptSeq s = prompt_seq(a, b);
   while (true) {
@@ -285,8 +286,7 @@ cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
   const int64_t blocks = (static_cast<int64_t>(a.max_q) * group + NW * 16 - 1) / (NW * 16);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(blocks, 1), 4096)), a.kv_heads,
                   std::min(a.num_seqs, 65535));
-  prompt_small_kernel<T, D, NW><<<grid, NW * 32, C::SMEM, stream>>>(a);
-  return cudaGetLastError();
+  return launch_after(prompt_small_kernel<T, D, NW>, grid, NW * 32, C::SMEM, stream, a.pdl, 1, a);
 }
 
 // ---- many query rows: tcgen05 -----------------------------------------------------
@@ -383,19 +383,6 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   const int group = a.heads / a.kv_heads;
   const int tpt = kPaRows / group;  // tokens of a tile
 
-  // ---- items of each thread's slice of sequences, and their prefix sums
-  const int slice = (a.num_seqs + kPaThreads - 1) / kPaThreads;
-  auto pairs_of = [&](int nq) { return (nq + 2 * tpt - 1) / (2 * tpt); };
-  int mine = 0;
-#pragma unroll 1
-  for (int b = tid * slice; b < min((tid + 1) * slice, a.num_seqs); ++b) mine += pairs_of(prompt_seq(a, b).nq) * a.kv_heads;
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(~0u, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) s_warp[warp] = incl;
   if (tid == 0) {
 #pragma unroll 1
     for (int i = 0; i < S; ++i) {
@@ -416,6 +403,21 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     fence_mbar_init();
   }
   if (warp == 0) tmem_alloc(s_tmem, 512);
+  pdl_wait_prior();
+
+  // ---- items of each thread's slice of sequences, and their prefix sums
+  const int slice = (a.num_seqs + kPaThreads - 1) / kPaThreads;
+  auto pairs_of = [&](int nq) { return (nq + 2 * tpt - 1) / (2 * tpt); };
+  int mine = 0;
+#pragma unroll 1
+  for (int b = tid * slice; b < min((tid + 1) * slice, a.num_seqs); ++b) mine += pairs_of(prompt_seq(a, b).nq) * a.kv_heads;
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(~0u, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_warp[warp] = incl;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -794,8 +796,8 @@ cudaError_t launch_tiles(int dtype, const PromptArgs& a, int num_sms, cudaStream
       !prompt_map(&maps.v, dtype, a.v, a.dim, a.kv_heads, a.k_tokens, a.v_ts, a.v_hs, 1, kPaKeys))
     return cudaErrorInvalidValue;
   const int64_t most = (static_cast<int64_t>(a.q_tokens) / (2 * tpt) + a.num_seqs) * a.kv_heads;
-  prompt_tile_kernel<T, DP><<<static_cast<unsigned>(std::min<int64_t>(num_sms, most)), kPaThreads, C::SMEM, stream>>>(a, maps);
-  return cudaGetLastError();
+  return launch_after(prompt_tile_kernel<T, DP>, dim3(static_cast<unsigned>(std::min<int64_t>(num_sms, most))), kPaThreads,
+                      C::SMEM, stream, a.pdl, 1, a, maps);
 }
 
 // The tiled kernel takes sequences that fill a good part of a tile, with

@@ -258,6 +258,7 @@ struct Kv4Args {
   float2* part_ml;  // their running maximum (log2 units) and sum, [2 per warp][rows]
   int4* part_desc;  // [warp][2]: the shared segment that starts in this warp's range
   int* err;
+  int pdl;  // 1: programmatic dependent launch
 };
 
 cudaError_t launch_kv4_append(int dtype, int head_dim, const Kv4Args& a, cudaStream_t stream);
@@ -284,6 +285,7 @@ struct LogprobArgs {
   float* entropy;  // or null
   int* top_ids;  // [rows][top]
   float* top_logprobs;
+  int pdl;
 };
 // dtype: WP_DTYPE_F16 / BF16 / F32
 cudaError_t launch_token_logprobs(int dtype, const LogprobArgs& a, int num_sms, cudaStream_t stream);
@@ -313,6 +315,7 @@ struct PromptArgs {
   int max_q;
   float scale;
   int* err;
+  int pdl;
 };
 cudaError_t launch_prompt_attention(int dtype, const PromptArgs& a, int num_sms, cudaStream_t stream);
 

@@ -117,6 +117,7 @@ __device__ __forceinline__ uint32_t code_of(float d, float step, float inv) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Kv4Args a, int per_seq) {
+  pdl_wait_prior();
   constexpr int TB = kv4_tile_bytes(D);
   constexpr int PER = D / 16;  // lanes per row
   constexpr int RW = 32 / PER;  // rows per warp; even warps take K, odd ones V
@@ -214,6 +215,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Kv4Args a, int
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Kv4Args a, int per_seq) {
+  pdl_wait_prior();
   constexpr int TB = kv4_tile_bytes(D);
   constexpr int PER = D / 16;
   __shared__ __align__(16) uint8_t tile[TB];
@@ -347,6 +349,10 @@ __global__ void __launch_bounds__(AttnCfg<D, NT>::THREADS, 1) kv4_attention_kern
   const int group = a.heads / a.kv_heads;
   const GroupDiv by(group);
 
+  if (lane < C::S) mbar_init(&bars[warp * C::S + lane], 1);
+  fence_mbar_init();
+  pdl_wait_prior();
+
   // ---- the call's chunks: each thread counts a contiguous slice of sequences
   const int slice = (a.num_seqs + kAttnThreads - 1) / kAttnThreads;
   auto seq_chunks = [&](int b) {
@@ -365,8 +371,6 @@ __global__ void __launch_bounds__(AttnCfg<D, NT>::THREADS, 1) kv4_attention_kern
   }
   __shared__ int s_warp[kAttnWarps];
   if (lane == 31) s_warp[warp] = incl;
-  if (lane < C::S) mbar_init(&bars[warp * C::S + lane], 1);
-  fence_mbar_init();
   __syncthreads();
   int before = 0, total = 0;
 #pragma unroll
@@ -816,70 +820,103 @@ __global__ void __launch_bounds__(AttnCfg<D, NT>::THREADS, 1) kv4_attention_kern
 }
 
 // Adds the partial rows of segments that several warps shared, in warp order.
-// A warp takes a quarter of one row's dimensions; its four lane groups take
-// every fourth part.
+// Most warps' ranges hold no start of such a segment, so descriptors are read
+// 32 at a time. A segment of few parts (the usual case with many sequences)
+// takes one warp per row, whose loads are all issued together; one of many
+// parts (few sequences) takes four, each a quarter of the dimensions.
+
 constexpr int kJoinWarps = 8;
+constexpr int kJoinFew = 16;  // parts that one warp joins
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv4_combine_kernel(const Kv4Args a, int warps) {
   using C = AttnCfg<D, NT>;
-  constexpr int Q = D / 4;  // dimensions per unit
-  constexpr int LANES = Q / 4;  // lanes per part: float4 each
-  constexpr int PARTS = 32 / LANES;  // parts at a time
-  pdl_wait_prior();
   const int lane = threadIdx.x & 31;
   const int group = a.heads / a.kv_heads;
-  // A warp has one (row, quarter) and every ngrp-th first warp of a segment;
-  // most of those have no shared segment, so their descriptors are read 32 at
-  // a time.
   const int gw = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
   const int quarter = gw & 3, row = (gw >> 2) % C::ROWS, grp = gw / (4 * C::ROWS);
   const int ngrp = gridDim.x * kJoinWarps / (4 * C::ROWS);
+  pdl_wait_prior();
   for (int base = grp; base < warps; base += ngrp * 32) {
-    const int4 mine = base + lane * ngrp < warps ? __ldcg(a.part_desc + 2 * (base + lane * ngrp)) : make_int4(0, 0, 0, 0);
-    for (unsigned todo = __ballot_sync(~0u, mine.x != 0 && row < mine.w); todo; todo &= todo - 1) {
+    const int w0 = base + lane * ngrp;
+    const int4 none = make_int4(0, 0, 0, 0);
+    const int4 m0 = w0 < warps ? __ldcg(a.part_desc + 2 * w0) : none, m1 = w0 < warps ? __ldcg(a.part_desc + 2 * w0 + 1) : none;
+    const bool mine = m0.x != 0 && row < m0.w && (m0.x > kJoinFew || (lane & 3) == quarter);
+    for (unsigned todo = __ballot_sync(~0u, mine); todo; todo &= todo - 1) {
       const int from = __ffs(todo) - 1, w = base + from * ngrp;
-      const int parts = __shfl_sync(~0u, mine.x, from), slot0 = 2 * w + __shfl_sync(~0u, mine.y, from);
-      const int first = __shfl_sync(~0u, mine.z, from);
-      const int4 d1 = __ldcg(a.part_desc + 2 * w + 1);
-      auto slot_of = [&](int i) { return i == 0 ? slot0 : 2 * (w + i); };
-      float top = -INFINITY;
-      for (int i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(a.part_ml + slot_of(i) * C::ROWS + row).x);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-      const float ref = top == -INFINITY ? 0.f : top;
-      float4 o4 = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
-      const int q = lane % LANES;
-#pragma unroll 8
-      for (int i = lane / LANES; i < parts; i += PARTS) {
-        const int64_t at = static_cast<int64_t>(slot_of(i)) * C::ROWS + row;
-        const float2 ml = __ldcg(a.part_ml + at);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part + at * D + quarter * Q) + q);
-        const float f = ex2(ml.x - ref);
-        sum += f * ml.y;
+      const int parts = __shfl_sync(~0u, m0.x, from), slot0 = 2 * w + __shfl_sync(~0u, m0.y, from);
+      const int first = __shfl_sync(~0u, m0.z, from), r = __shfl_sync(~0u, m1.x, from) + row;
+      const int h = __shfl_sync(~0u, m1.y, from);
+      auto at = [&](int i) { return static_cast<int64_t>(i == 0 ? slot0 : 2 * (w + i)) * C::ROWS + row; };
+      const int64_t to = (static_cast<int64_t>(first) + r / group) * a.heads + h * group + r % group;
+      auto put = [&](int d, float4 o, float sum) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + to * D + d) =
+            make_uint2(Elem<T>::pack2(o.x * inv, o.y * inv), Elem<T>::pack2(o.z * inv, o.w * inv));
+      };
+      auto add = [&](float4& o, float f, float4 v) {
         if (f != 0.f) {  // a part that saw nothing adds nothing
-          o4.x += f * v.x;
-          o4.y += f * v.y;
-          o4.z += f * v.z;
-          o4.w += f * v.w;
+          o.x += f * v.x;
+          o.y += f * v.y;
+          o.z += f * v.z;
+          o.w += f * v.w;
         }
-      }
+      };
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f, top = -INFINITY;
+      if (parts <= kJoinFew) {
+        const int d = lane * 4;
+        const float2 ml = lane < parts ? __ldcg(a.part_ml + at(lane)) : make_float2(-INFINITY, 0.f);
+        float4 v[kJoinFew / 2];
+        auto load = [&](int i0) {
 #pragma unroll
-      for (int o = LANES; o < 32; o <<= 1) {
-        sum += __shfl_xor_sync(~0u, sum, o);
-        o4.x += __shfl_xor_sync(~0u, o4.x, o);
-        o4.y += __shfl_xor_sync(~0u, o4.y, o);
-        o4.z += __shfl_xor_sync(~0u, o4.z, o);
-        o4.w += __shfl_xor_sync(~0u, o4.w, o);
+          for (int i = 0; i < kJoinFew / 2; ++i)
+            if (i0 + i < parts && d < D) v[i] = __ldcg(reinterpret_cast<const float4*>(a.part + at(i0 + i) * D + d));
+        };
+        load(0);
+        top = ml.x;
+#pragma unroll
+        for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+        const float f = ex2(ml.x - (top == -INFINITY ? 0.f : top));
+        sum = f * ml.y;
+#pragma unroll
+        for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(~0u, sum, s);
+        for (int i0 = 0; i0 < parts; i0 += kJoinFew / 2) {
+          if (i0 > 0) load(i0);
+#pragma unroll
+          for (int i = 0; i < kJoinFew / 2; ++i) {
+            const float fi = __shfl_sync(~0u, f, (i0 + i) & 31);
+            if (i0 + i < parts) add(o, fi, v[i]);
+          }
+        }
+        if (d < D) put(d, o, sum);
+      } else {
+        constexpr int LANES = D / 16, PARTS = 32 / LANES;  // a quarter of the dimensions; parts at a time
+        const int d = quarter * (D / 4) + lane % LANES * 4;
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(a.part_ml + at(i)).x);
+#pragma unroll
+        for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 8
+        for (int i = lane / LANES; i < parts; i += PARTS) {
+          const float2 ml = __ldcg(a.part_ml + at(i));
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part + at(i) * D + d));
+          const float f = ex2(ml.x - ref);
+          sum += f * ml.y;
+          add(o, f, v);
+        }
+#pragma unroll
+        for (int s = LANES; s < 32; s <<= 1) {
+          sum += __shfl_xor_sync(~0u, sum, s);
+          o.x += __shfl_xor_sync(~0u, o.x, s);
+          o.y += __shfl_xor_sync(~0u, o.y, s);
+          o.z += __shfl_xor_sync(~0u, o.z, s);
+          o.w += __shfl_xor_sync(~0u, o.w, s);
+        }
+        if (lane < LANES) put(d, o, sum);
       }
-      const int r = d1.x + row;
-      const int64_t at = (static_cast<int64_t>(first) + r / group) * a.heads + d1.y * group + r % group;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      if (lane < LANES)
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * D + quarter * Q + q * 4) =
-            make_uint2(Elem<T>::pack2(o4.x * inv, o4.y * inv), Elem<T>::pack2(o4.z * inv, o4.w * inv));
-      if (a.lse && quarter == 0 && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+      if (a.lse && (parts <= kJoinFew || quarter == 0) && lane == 0)
+        a.lse[to] = sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + __log2f(sum)) * kLn2;
     }
   }
 }
@@ -917,19 +954,11 @@ struct Attn {
     a.part_desc = static_cast<int4*>(ws);
     a.part = reinterpret_cast<float*>(a.part_desc + 2 * warps);
     a.part_ml = reinterpret_cast<float2*>(a.part + 2 * warps * C::ROWS * D);
-    kv4_attention_kernel<T, D, NT><<<grid, C::THREADS, C::SMEM, stream>>>(a);
-    cudaError_t e = cudaGetLastError();
+    cudaError_t e = launch_after(kv4_attention_kernel<T, D, NT>, dim3(grid), C::THREADS, C::SMEM, stream, a.pdl, 1, a);
     if (e != cudaSuccess) return e;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(num_sms * 8);  // 8 warps each: every shared row's quarter finds a warp of its own
-    cfg.blockDim = dim3(kJoinWarps * 32);
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D, NT>, a, static_cast<int>(warps));
+    // 8 CTAs per SM: nearly every shared row finds a warp of its own
+    return launch_after(kv4_combine_kernel<T, D, NT>, dim3(num_sms * 8), kJoinWarps * 32, 0, stream, a.pdl, 1, a,
+                        static_cast<int>(warps));
   }
 };
 
@@ -952,16 +981,14 @@ template <typename T, int D>
 struct Append {
   static cudaError_t run(const Kv4Args& a, cudaStream_t stream) {
     const int per = move_per_seq(a);
-    kv4_append_kernel<T, D><<<dim3(a.num_seqs * per, a.kv_heads), kMoveThreads, 0, stream>>>(a, per);
-    return cudaGetLastError();
+    return launch_after(kv4_append_kernel<T, D>, dim3(a.num_seqs * per, a.kv_heads), kMoveThreads, 0, stream, a.pdl, 1, a, per);
   }
 };
 template <typename T, int D>
 struct Read {
   static cudaError_t run(const Kv4Args& a, cudaStream_t stream) {
     const int per = move_per_seq(a);
-    kv4_read_kernel<T, D><<<dim3(a.num_seqs * per, a.kv_heads), kMoveThreads, 0, stream>>>(a, per);
-    return cudaGetLastError();
+    return launch_after(kv4_read_kernel<T, D>, dim3(a.num_seqs * per, a.kv_heads), kMoveThreads, 0, stream, a.pdl, 1, a, per);
   }
 };
 template <typename T, int D>

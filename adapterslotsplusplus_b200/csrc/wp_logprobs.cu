@@ -35,15 +35,9 @@ namespace wp {
 namespace {
 
 constexpr int kLpThreads = 256;
-#ifndef LP_PER
-#define LP_PER 4
-#endif
-constexpr int kLpPerSm = LP_PER;  // CTAs of one SM
+constexpr int kLpPerSm = 4;  // CTAs of one SM (64 registers; 5 and 6 measured the same or slower)
 constexpr int kLpWarps = kLpThreads / 32;
-#ifndef LP_AHEAD
-#define LP_AHEAD 4
-#endif
-constexpr int kLpAhead = LP_AHEAD;  // vectors that a thread has in flight
+constexpr int kLpAhead = 4;  // vectors that a thread has in flight
 constexpr int kLpCands = 1024;  // candidates for the alternatives in one CTA
 
 // 16 bytes of logits as fp32.
@@ -213,27 +207,22 @@ __device__ __forceinline__ void for_row(const Row<T>& row, int rank, int ranks, 
   // the next kLpAhead vectors load while these are worked on; those past the
   // end count as minus infinity
   uint4 x[kLpAhead];
-  auto load = [&](int i, bool inside) {
+  auto load = [&](int i) {
 #pragma unroll
     for (int j = 0; j < kLpAhead; ++j)
-      x[j] = inside || i + j * step < row.nvec ? row.vec(i + j * step)
-                                               : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+      x[j] = i + j * step < row.nvec ? row.vec(i + j * step) : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
   };
   int i = rank * kLpThreads + threadIdx.x;
-  load(i, false);
-  auto work = [&](bool inside) {
+  load(i);
+#pragma unroll 1
+  for (; i < row.nvec; i += kLpAhead * step) {
     uint4 y[kLpAhead];
 #pragma unroll
     for (int j = 0; j < kLpAhead; ++j) y[j] = x[j];
-    load(i + kLpAhead * step, inside);
+    load(i + kLpAhead * step);
 #pragma unroll
     for (int j = 0; j < kLpAhead; ++j) g(y[j], row.head + (i + j * step) * N);
-    i += kLpAhead * step;
-  };
-#pragma unroll 1
-  while (i + (2 * kLpAhead - 1) * step < row.nvec) work(true);
-#pragma unroll 1
-  while (i < row.nvec) work(false);
+  }
   if (rank == ranks - 1) {
     const int t = threadIdx.x;
     if (t < row.head) f(load1(row.p + t), t);
@@ -244,7 +233,7 @@ __device__ __forceinline__ void for_row(const Row<T>& row, int rank, int ranks, 
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(const LogprobArgs a) {
   constexpr int N = Vec<T>::N;
-  __shared__ Stat s_stat[kLpWarps];
+  __shared__ Stat s_stat[kLpWarps], s_all;
   __shared__ uint32_t s_max[kLpThreads];  // each thread's maximum
   __shared__ unsigned long long s_cand[kLpCands], s_top[kMaxTop], s_best[kLpWarps];
   __shared__ uint16_t s_hit[kLpThreads];
@@ -253,6 +242,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   __shared__ Share s_share[8];  // on the cluster's first CTA: every CTA's result
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+  pdl_wait_prior();
   if (ranks > 1) cluster_arrive();  // every CTA runs before the first one's shared memory is written
   const int64_t t = blockIdx.x / ranks;
   const Row<T> row(static_cast<const T*>(a.logits) + t * a.ld, a.vocab);
@@ -317,6 +307,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   for (int o = 16; o; o >>= 1) w = merge(w, shfl_xor(w, o));
   if (lane == 0) s_stat[warp] = w;
   if (tid == 0) s_ncand = s_nhit = 0;
+  if (tid < kMaxTop) s_top[tid] = 0;
   __syncthreads();
   if (a.top > 0 && warp == 0) {
     // 32 groups of threads: the top-th largest of their maxima (0: fewer have one)
@@ -330,10 +321,14 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
       place += o > mine || (o == mine && i < lane);
     }
     if (place == a.top - 1) s_bound = mine;
-  }
-  w = s_stat[0];
+  } else if (warp == kLpWarps - 1) {
+    w = s_stat[lane % kLpWarps];
 #pragma unroll
-  for (int i = 1; i < kLpWarps; ++i) w = merge(w, s_stat[i]);
+    for (int o = kLpWarps / 2; o; o >>= 1) w = merge(w, shfl_xor(w, o));
+    if (lane == 0) s_all = w;
+  }
+  __syncthreads();
+  w = s_all;
   // Where nothing is well above the lowest logit (masked rows), or the maximum
   // is enormous, the sums again with x - M exact: M is known now.
   if (!(w.raw > Vec<T>::kLow + 200.f && w.raw < 1e38f) && w.raw < INFINITY && w.l == w.l) {
@@ -352,7 +347,6 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
 #pragma unroll
           for (int i = 0; i < N; ++i) exact(x[i]);
         });
-    __syncthreads();  // s_stat was read
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       l += __shfl_xor_sync(~0u, l, o);
@@ -374,8 +368,6 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   // ---- the largest `top` of this CTA's part of the row
   unsigned long long mine = 0;  // thread i < top: the i-th largest key
   if (a.top > 0) {
-    if (tid < kMaxTop) s_top[tid] = 0;
-    __syncthreads();
     const uint32_t bound = s_bound;
     const float low = bound == 0 ? -INFINITY : unordered(bound);
     auto keep = [&](float x, int i) {
@@ -506,17 +498,7 @@ cudaError_t launch(const LogprobArgs& a, int num_sms, cudaStream_t stream) {
   while (ranks < 8 && static_cast<int64_t>(a.rows) * 2 * ranks <= kLpPerSm * num_sms &&
          static_cast<int64_t>(a.vocab) >= static_cast<int64_t>(2 * ranks) * kLpThreads * Vec<T>::N)
     ranks *= 2;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.rows * ranks);
-  cfg.blockDim = dim3(kLpThreads);
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a);
+  return launch_after(token_logprobs_kernel<T>, dim3(a.rows * ranks), kLpThreads, 0, stream, a.pdl, ranks, a);
 }
 
 }  // namespace
