@@ -328,9 +328,10 @@ constexpr int kPaKeys = 128;  // keys of a block
 constexpr float kPaLazy = 8.f;
 // Of 8 pairs of weights, those that take the FMA pipe instead of the special-
 // function unit. 8192 tokens, 32 query / 8 kv heads of 128, bf16: 493, 498, 450
-// and 481 us for 0, 1, 2 and 3 (1.22 PFLOP/s, 74% of the measured matrix rate;
-// what bounds it is the chain scores -> maximum -> weights -> products of a
-// tile, 3000-3500 cycles per 128 keys against 2100 of the products themselves).
+// and 481 us for 0, 1, 2 and 3 in single calls (1.22 PFLOP/s, 74% of the
+// measured matrix rate), 555, 580, 568 and more back to back under the power
+// cap. What bounds it is the chain scores -> maximum -> weights -> products of
+// a tile, 3000-3500 cycles per 128 keys against 2100 of the products alone.
 constexpr int kPaFma = 2;
 
 template <int DP>

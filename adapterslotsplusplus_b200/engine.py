@@ -430,16 +430,19 @@ class WarpPipeEngine:
         if not tokens.is_contiguous():
             tokens = tokens.contiguous()
         dev = logits.device
-        f = torch.empty(rows * (2 + top), dtype=torch.float32, device=dev)
-        i = torch.empty(rows * (1 + top), dtype=torch.int32, device=dev)
-        fp, ip = f.data_ptr(), i.data_ptr()
+        # one allocation: log probabilities, entropies, the alternatives' log
+        # probabilities; ranks, the alternatives' ids
+        buf = torch.empty(rows * (3 + 2 * top), dtype=torch.float32, device=dev)
+        p, r, t = buf.data_ptr(), 4 * rows, 4 * rows * top
         self._check(self._lib.wp_token_logprobs(
-            self._h, fp, ip, fp + 4 * rows, ip + 4 * rows, fp + 8 * rows, logits.data_ptr(), max(ld, vocab),
+            self._h, p, p + 2 * r + t, p + r, p + 3 * r + t, p + 2 * r, logits.data_ptr(), max(ld, vocab),
             tokens.data_ptr(), _lib.WP_DTYPE_I64 if tokens.dtype == torch.int64 else _lib.WP_DTYPE_I32, rows, vocab, top,
             code, _stream_ptr(dev)))
-        logprob, entropy, top_logprobs = f.split((rows, rows, rows * top))
-        rank, top_ids = i.split((rows, rows * top))
-        return TokenLogprobs(logprob, rank, entropy, top_ids.view(rows, top), top_logprobs.view(rows, top))
+        whole, view = buf.view(torch.int32), torch.as_strided
+        n = rows * top
+        return TokenLogprobs(view(buf, (rows,), (1,)), view(whole, (rows,), (1,), 2 * rows + n),
+                             view(buf, (rows,), (1,), rows), view(whole, (rows, top), (top, 1), 3 * rows + n),
+                             view(buf, (rows, top), (top, 1), 2 * rows))
 
     # -- staging slots (engine.py:44-54) -----------------------------------------
     def prefetch_adapter(self, adapter_id) -> int:

@@ -108,12 +108,13 @@ class KvCache4:
             tokens = int(lens.numel())
         tokens = int(tokens)
         table, lens, cu, n = self._place(table, lens, cu, tokens, "read")
-        k = torch.empty(tokens, self.kv_heads, self.head_dim, dtype=self.dtype, device=self.pages.device)
+        dev = self.pages.device
+        k = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=self.dtype, device=dev)
         v = torch.empty_like(k)
         _lib.check(self._lib.wp_kv4_read(
             self.engine.handle, k.data_ptr(), v.data_ptr(), self.pages.data_ptr(), self.num_pages, self.page_size,
             table.data_ptr(), table.size(1), lens.data_ptr(), None if cu is None else cu.data_ptr(), n, tokens,
-            self.kv_heads, self.head_dim, self._code, _stream_ptr(self.pages.device)), self.engine.handle)
+            self.kv_heads, self.head_dim, self._code, _stream_ptr(dev)), self.engine.handle)
         return k, v
 
     def attention(self, q: torch.Tensor, table, lens, cu=None, max_q: int = 1, scale: Optional[float] = None,
