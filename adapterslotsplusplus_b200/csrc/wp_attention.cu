@@ -801,15 +801,22 @@ cudaError_t launch_tiles(int dtype, const PromptArgs& a, int num_sms, cudaStream
                       C::SMEM, stream, a.pdl, 1, a, maps);
 }
 
-// The tiled kernel takes sequences that fill a good part of a tile, with
-// strides a tensor map can express; its maxima are of unscaled scores, so the
-// scale has to be positive.
+// The tiled kernel takes sequences of more than one tile of packed rows, and
+// shorter ones over long contexts, whose keys are what counts. Measured, tiled
+// against warp-level kernel (bf16): 64 sequences of 4 / 64 / 128 tokens, 12
+// heads of 64: 25.9 / 26.1 / 28.7 against 5.2 / 10.3 / 21.6 us; 16 sequences,
+// 32 query / 8 kv heads of 128, of 32 / 64 tokens (128 / 256 rows): 9.4 / 11.8
+// against 6.3 / 13.5 us; 4 tokens behind 2000 keys: 34 against 113 us, 64 rows
+// behind 500 keys: 59 against 43 us. It needs strides that a tensor map can
+// express, and a positive scale, because its maxima are of unscaled scores.
+constexpr int64_t kTileRows = 128, kTileKeys = 1024;
+
 bool use_tiles(const PromptArgs& a) {
   const int group = a.heads / a.kv_heads;
   const int64_t rows = static_cast<int64_t>(a.max_q) * group;
   const int64_t most = int64_t{1} << 38;
   auto ok = [&](int64_t s) { return s > 0 && s < most; };
-  return rows >= 64 && group <= kPaRows && a.k_tokens > 0 && a.scale > 0.f && a.scale < 1e30f && ok(a.q_ts) && ok(a.q_hs) &&
+  return (rows > kTileRows || a.k_tokens >= kTileKeys * a.num_seqs) && group <= kPaRows && a.k_tokens > 0 && a.scale > 0.f && a.scale < 1e30f && ok(a.q_ts) && ok(a.q_hs) &&
          ok(a.k_ts) && ok(a.k_hs) && ok(a.v_ts) && ok(a.v_hs);
 }
 
