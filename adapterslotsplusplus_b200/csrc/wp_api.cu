@@ -2242,7 +2242,7 @@ int wp_prompt_attention(wp_handle* h, void* out, float* lse, const void* q, int6
   a.err = h->d_err;
   a.pdl = h->cfg.use_pdl;
   DeviceGuard dg(h->device);
-  cudaError_t e = wp::launch_prompt_attention(dtype, a, h->num_sms, static_cast<cudaStream_t>(stream));
+  cudaError_t e = wp::launch_prompt_attention(dtype, a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(h, WP_ERR_CUDA, "prompt_attention launch: %s", cudaGetErrorString(e));
   ++h->launches;
   return WP_OK;

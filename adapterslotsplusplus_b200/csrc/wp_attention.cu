@@ -97,7 +97,9 @@ __device__ __forceinline__ void cp_async_wait() {
 //
 // NW warps share 64-key tiles of K and V (two of each, loaded asynchronously);
 // a warp has 16 packed rows. For sequences of a few tokens, where a tcgen05
-// tile of 128 rows would be nearly empty and latency is everything.
+// tile of 128 rows would be nearly empty and latency is everything: 5 us for 64
+// sequences of 4 tokens, 12 heads of 64 (0.24 us of traffic), of which about 4
+// are the launch and three dependent loads (offsets, tiles, result).
 
 template <typename T, int D, int NW>
 struct SmallCfg {
@@ -300,8 +302,8 @@ cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
 //
 // Warps (384 threads): 0-3 softmax of tile 0, 4-7 of tile 1 (one thread per
 // row: no exchange between lanes), 8 TMA producer, 9 and 10 MMA issuers of tile
-// 0 and 1; 11 only gives its registers to the softmax warps, which hold a row's
-// 128 scores (256 x 216 + 128 x 72 = the launch's 384 x 168). While one tile's
+// 0 and 1, 11 fetches items. The last four give registers to the softmax warps,
+// which hold a row's 128 scores (256 x 216 + 128 x 72 = the launch's 384 x 168). While one tile's
 // softmax runs, the other's P V and next Q K^T keep the tensor core busy. Each
 // tile has its own issuer because the tensor core queues only a few products,
 // so one issuer's waits for both tiles would drain it; the issuers take turns
@@ -315,9 +317,18 @@ cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
 // log2 units): weights then reach 2^8 at most, which costs fp16 and bf16
 // nothing, and O is rescaled in a few blocks at the start instead of in most.
 //
-// Persistent: CTA c takes items c, 2 G - 1 - c, 2 G + c, ... in the order
-// (sequence, pairs from the last one, kv head), so long items come first
-// within a sequence and every CTA gets its share of them.
+// The grid has a CTA per item, in the order (sequence, pairs from the last one,
+// kv head), so long items come first within a sequence. A resident CTA that
+// has issued an item's last load cancels the launch of one of the CTAs that
+// still wait for an SM and takes over its item next (warp 11, which also looks
+// it up for the others). So an SM is set up once, its next item's loads run
+// while the current one ends, and no SM is left with two long items at the end.
+// Against one CTA per SM with a fixed share of the items, which every warp
+// looked up for itself (32 query / 8 kv heads of 128, device time): 4 sequences
+// of 2048 tokens 151 against 204 us, 64 of 100-400 tokens 123 / 136, one of
+// 8192 469 / 499, 16 of 1-1500 tokens 42.3 / 50.4; 64 of 256, 12 heads of 64:
+// 38 / 44. Taking the next item when the current one begins: 159, 123, 474,
+// 50.7 and 38 us; two ahead, 175 us in the first case.
 
 constexpr int kPaWarps = 12;
 constexpr int kPaThreads = kPaWarps * 32;
@@ -327,11 +338,12 @@ constexpr int kPaRows = 128;  // rows of a tile
 constexpr int kPaKeys = 128;  // keys of a block
 constexpr float kPaLazy = 8.f;
 // Of 8 pairs of weights, those that take the FMA pipe instead of the special-
-// function unit. 8192 tokens, 32 query / 8 kv heads of 128, bf16: 493, 498, 450
-// and 481 us for 0, 1, 2 and 3 in single calls (1.22 PFLOP/s, 74% of the
-// measured matrix rate), 555, 580, 568 and more back to back under the power
-// cap. What bounds it is the chain scores -> maximum -> weights -> products of
-// a tile, 3000-3500 cycles per 128 keys against 2100 of the products alone.
+// function unit. 32 query / 8 kv heads of 128, bf16, for 1, 2 and 3: 4 x 2048
+// tokens 158, 151 and 152 us, 64 x 100-400 tokens 126, 123 and 126, 1 x 8192
+// 478, 472 and 467 (1.17 PFLOP/s, 70% of the measured matrix rate). What bounds
+// it is the chain scores -> maximum -> weights -> products of a tile, 3000-3500
+// cycles per 128 keys against 2100 of the products alone; in long runs also the
+// power cap.
 constexpr int kPaFma = 2;
 
 template <int DP>
@@ -351,10 +363,10 @@ struct PaMaps {
   CUtensorMap k, v;  // [tokens][kv heads][dim], box 64 columns x 1 x 128
 };
 
-struct PaItem {
+struct __align__(16) PaItem {
   PromptSeq s;
   int kvh;
-  int t0;  // first token of the pair
+  int t0;  // first token of the pair; -1: no item any more
   int n[2];  // key blocks of each tile (0: no tokens, or none that sees a key)
 };
 
@@ -376,6 +388,11 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   uint64_t* o_free = kv_full + 30;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(kv_full + 32);
   volatile int* s_bad = reinterpret_cast<volatile int*>(kv_full + 33);
+  uint64_t* next_full = kv_full + 40;  // *s_item is the next item
+  uint64_t* next_empty = kv_full + 41;
+  uint64_t* taken = kv_full + 42;  // a cancellation's answer is there
+  uint4* s_answer = reinterpret_cast<uint4*>(kv_full + 44);
+  PaItem* s_item = reinterpret_cast<PaItem*>(kv_full + 46);
   int* s_warp = reinterpret_cast<int*>(kv_full + 34);  // [kPaWarps]
   int* s_sum = reinterpret_cast<int*>(smem + 512);  // items before thread i's slice of sequences
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + C::HEAD + 1023) & ~uintptr_t(1023));
@@ -400,6 +417,9 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       mbar_init(&o_full[i], 1);
       mbar_init(&o_free[i], 4);
     }
+    mbar_init(next_full, 1);
+    mbar_init(next_empty, kPaWarps - 1);
+    mbar_init(taken, 1);
     *s_bad = 0;
     fence_mbar_init();
   }
@@ -432,36 +452,16 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   s_sum[tid] = before + incl - mine;
   __syncthreads();
 
-  // The warp's n-th item; false past the last one.
+  // Waits for the CTA's n-th item, a whole warp together; false past the last one.
   auto item = [&](int n, PaItem& it) {
-    const int G = gridDim.x, x = n * G + (n & 1 ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
-    if (n * G >= total) return false;
-    if (x >= total) {  // the last round's tail: nothing for this CTA
-      it.n[0] = it.n[1] = -1;
-      return true;
+    if (!mbar_wait_warp(smem_u32(next_full), n & 1, a.err)) {
+      *s_bad = 1;
+      return false;
     }
-    int sl = 0;
-#pragma unroll 1
-    for (int i = lane; i < kPaThreads; i += 32)
-      if (s_sum[i] <= x) sl = i;
-    sl = __reduce_max_sync(~0u, sl);
-    int b = sl * slice, y = x - s_sum[sl], pairs;
-    while (true) {
-      it.s = prompt_seq(a, b);
-      pairs = pairs_of(it.s.nq);
-      if (y < pairs * a.kv_heads) break;
-      y -= pairs * a.kv_heads;
-      ++b;
-    }
-    it.kvh = y % a.kv_heads;
-    it.t0 = (pairs - 1 - y / a.kv_heads) * 2 * tpt;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int first = it.t0 + i * tpt, last = min(first + tpt, it.s.nq) - 1;
-      const int end = first < it.s.nq ? min(max(last + it.s.nk - it.s.nq + 1, 0), it.s.nk) : 0;
-      it.n[i] = (end + kPaKeys - 1) / kPaKeys;
-    }
-    return true;
+    it = *s_item;
+    __syncwarp();
+    if (lane == 0 && warp != kPaProd) mbar_arrive(next_empty);
+    return it.t0 >= 0;
   };
 
   PaItem it;
@@ -502,6 +502,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
                           it.s.k0 + (j >> 1) * kPaKeys, &kv_full[st]);
           }
         }
+        if (lane == 0) mbar_arrive(next_empty);
         __syncwarp();
       }
       if (lane == 0 && *s_bad)  // a wait ran out: let the copies in flight land before the CTA leaves
@@ -615,6 +616,59 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         if (elect_one()) umma_commit_at(bar(o_full) + 8 * i);
         mbar_wait_bounded(o_full + i, 0, a.err, 1000000ull);
       }
+    } else {
+      // ============================ items ====================================
+      // Fetched when every warp has begun the current one and its last load has
+      // been issued.
+      uint32_t par = 0;
+#pragma unroll 1
+      for (int n = 0, x = blockIdx.x; x >= 0; ++n) {
+        if (lane == 0) {
+          bool ok = n == 0 || mbar_wait_bounded(next_empty, (n - 1) & 1, a.err);
+          for (bool more = n > 0; ok && (more || x >= total); more = false) {
+            mbar_arrive_expect_tx(taken, 16);
+            cancel_cta(s_answer, taken);
+            ok = mbar_wait_bounded(taken, par, a.err);
+            par ^= 1;
+            if (ok) x = cancelled_cta(s_answer);
+            fence_proxy_async_smem();  // read before the next answer is written
+          }
+          if (!ok) {
+            *s_bad = 1;
+            x = -1;
+          }
+        }
+        x = __shfl_sync(~0u, x, 0);
+        it.t0 = -1;
+        if (x >= 0) {
+          int sl = 0;
+#pragma unroll 1
+          for (int i = lane; i < kPaThreads; i += 32)
+            if (s_sum[i] <= x) sl = i;
+          sl = __reduce_max_sync(~0u, sl);
+          int b = sl * slice, y = x - s_sum[sl], pairs;
+          while (true) {
+            it.s = prompt_seq(a, b);
+            pairs = pairs_of(it.s.nq);
+            if (y < pairs * a.kv_heads) break;
+            y -= pairs * a.kv_heads;
+            ++b;
+          }
+          it.kvh = y % a.kv_heads;
+          it.t0 = (pairs - 1 - y / a.kv_heads) * 2 * tpt;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int first = it.t0 + i * tpt, last = min(first + tpt, it.s.nq) - 1;
+            const int end = first < it.s.nq ? min(max(last + it.s.nk - it.s.nq + 1, 0), it.s.nk) : 0;
+            it.n[i] = (end + kPaKeys - 1) / kPaKeys;
+          }
+        }
+        if (lane == 0) {
+          *s_item = it;
+          mbar_arrive(next_full);
+        }
+        __syncwarp();
+      }
     }
   } else {
     // ============================ softmax, one thread per row ================
@@ -628,7 +682,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     for (int n = 0; item(n, it) && __all_sync(~0u, !*s_bad); ++n) {
       const int first = it.t0 + i * tpt;
       const int blocks = i ? it.n[1] : it.n[0];
-      if (blocks < 0 || first >= it.s.nq) continue;
+      if (first >= it.s.nq) continue;
       const int token = first + row / group, head = it.kvh * group + row % group;
       const bool live = row < tpt * group && token < it.s.nq;
       const int shift = it.s.nk - it.s.nq + 1;
@@ -782,7 +836,7 @@ bool prompt_map(CUtensorMap* m, int dtype, const void* base, int dim, int heads,
 }
 
 template <typename T, int DP>
-cudaError_t launch_tiles(int dtype, const PromptArgs& a, int num_sms, cudaStream_t stream) {
+cudaError_t launch_tiles(int dtype, const PromptArgs& a, cudaStream_t stream) {
   using C = PaCfg<DP>;
   static std::atomic<bool> ready{false};
   if (!ready.load()) {
@@ -796,9 +850,12 @@ cudaError_t launch_tiles(int dtype, const PromptArgs& a, int num_sms, cudaStream
       !prompt_map(&maps.k, dtype, a.k, a.dim, a.kv_heads, a.k_tokens, a.k_ts, a.k_hs, 1, kPaKeys) ||
       !prompt_map(&maps.v, dtype, a.v, a.dim, a.kv_heads, a.k_tokens, a.v_ts, a.v_hs, 1, kPaKeys))
     return cudaErrorInvalidValue;
-  const int64_t most = (static_cast<int64_t>(a.q_tokens) / (2 * tpt) + a.num_seqs) * a.kv_heads;
-  return launch_after(prompt_tile_kernel<T, DP>, dim3(static_cast<unsigned>(std::min<int64_t>(num_sms, most))), kPaThreads,
-                      C::SMEM, stream, a.pdl, 1, a, maps);
+  // The items are not known here: their bound (768 CTAs too many cost nothing
+  // that was measured; too few, and their items fall to CTAs that have one).
+  const int64_t ctas = (static_cast<int64_t>(a.q_tokens) / (2 * tpt) + a.num_seqs) * a.kv_heads;
+  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  return launch_after(prompt_tile_kernel<T, DP>, dim3(static_cast<unsigned>(ctas)), kPaThreads, C::SMEM, stream, a.pdl, 1, a,
+                      maps);
 }
 
 // The tiled kernel takes sequences of more than one tile of packed rows, and
@@ -816,14 +873,14 @@ bool use_tiles(const PromptArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.max_q) * group;
   const int64_t most = int64_t{1} << 38;
   auto ok = [&](int64_t s) { return s > 0 && s < most; };
-  return (rows > kTileRows || a.k_tokens >= kTileKeys * a.num_seqs) && group <= kPaRows && a.k_tokens > 0 && a.scale > 0.f && a.scale < 1e30f && ok(a.q_ts) && ok(a.q_hs) &&
-         ok(a.k_ts) && ok(a.k_hs) && ok(a.v_ts) && ok(a.v_hs);
+  return (rows > kTileRows || a.k_tokens >= kTileKeys * a.num_seqs) && group <= kPaRows && a.k_tokens > 0 &&
+         a.scale > 0.f && a.scale < 1e30f && ok(a.q_ts) && ok(a.q_hs) && ok(a.k_ts) && ok(a.k_hs) && ok(a.v_ts) && ok(a.v_hs);
 }
 
 template <typename T>
-cudaError_t launch_prompt(int dtype, const PromptArgs& a, int num_sms, cudaStream_t stream) {
+cudaError_t launch_prompt(int dtype, const PromptArgs& a, cudaStream_t stream) {
   if (use_tiles(a))
-    return a.dim <= 64 ? launch_tiles<T, 64>(dtype, a, num_sms, stream) : launch_tiles<T, 128>(dtype, a, num_sms, stream);
+    return a.dim <= 64 ? launch_tiles<T, 64>(dtype, a, stream) : launch_tiles<T, 128>(dtype, a, stream);
   const int64_t rows = static_cast<int64_t>(a.max_q) * (a.heads / a.kv_heads);
   if (a.dim <= 64)
     return rows <= 16 ? launch_small<T, 64, 1>(a, stream) : launch_small<T, 64, 4>(a, stream);
@@ -832,9 +889,9 @@ cudaError_t launch_prompt(int dtype, const PromptArgs& a, int num_sms, cudaStrea
 
 }  // namespace
 
-cudaError_t launch_prompt_attention(int dtype, const PromptArgs& a, int num_sms, cudaStream_t stream) {
-  return dtype == 1 ? launch_prompt<__nv_bfloat16>(dtype, a, num_sms, stream)
-                    : launch_prompt<__half>(dtype, a, num_sms, stream);
+cudaError_t launch_prompt_attention(int dtype, const PromptArgs& a, cudaStream_t stream) {
+  return dtype == 1 ? launch_prompt<__nv_bfloat16>(dtype, a, stream)
+                    : launch_prompt<__half>(dtype, a, stream);
 }
 
 }  // namespace wp

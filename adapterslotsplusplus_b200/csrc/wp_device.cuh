@@ -440,6 +440,31 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// Asks for one CTA of this grid that has not been launched yet: its launch is
+// cancelled and the caller does its work. The 16-byte answer arrives in shared
+// memory and completes 16 bytes on the barrier. Not to be asked again after a
+// negative answer.
+__device__ __forceinline__ void cancel_cta(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The cancelled CTA's blockIdx.x, -1 for none.
+__device__ __forceinline__ int cancelled_cta(const void* answer) {
+  int x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}"
+      : "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return x;
+}
+
 // Shared-memory matrix descriptor of a K-major operand tile written in the
 // TMA swizzle `layout` (2 = 128B, 4 = 64B, 6 = 32B rows): start address,
 // leading offset 16 B (unused for swizzled K-major), stride `sbo` bytes

@@ -317,6 +317,6 @@ struct PromptArgs {
   int* err;
   int pdl;
 };
-cudaError_t launch_prompt_attention(int dtype, const PromptArgs& a, int num_sms, cudaStream_t stream);
+cudaError_t launch_prompt_attention(int dtype, const PromptArgs& a, cudaStream_t stream);
 
 }  // namespace wp
