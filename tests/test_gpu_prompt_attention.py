@@ -220,3 +220,17 @@ def test_refusals(eng):
             pytest.fail(f"call {i} was accepted")
     assert eng._lib.wp_prompt_attention(None, *[None] * 3, 0, 0, None, 0, 0, None, 0, 0, None, None, 1, 1, 1, 1, 1, 1, 64,
                                         0.1, 1, None) == -1
+
+
+@pytest.mark.parametrize("nq", [[0] * 700 + [300] + [0] * 700, [1, 0, 2] * 300 + [700], [260] * 90, [1500] + [30] * 200])
+def test_far_fewer_and_far_more_items_than_sms(eng, nq):
+    check(eng, nq, nq, 8, 8, 64, torch.bfloat16, max_q=max(nq))
+    check(eng, nq, [n + 3 if n else 0 for n in nq], 12, 4, 128, torch.float16, max_q=max(nq))
+
+
+def test_which_cta_takes_an_item_does_not_change_results(eng):
+    nq = [900, 1, 400, 650, 33, 1200]
+    q, k, v = (torch.randn(sum(nq), h, 128, device="cuda", dtype=torch.bfloat16) for h in (16, 4, 4))
+    first = eng.prompt_attention(q, k, v, starts(nq), max_q=max(nq))
+    for _ in range(10):
+        assert torch.equal(eng.prompt_attention(q, k, v, starts(nq), max_q=max(nq)), first)
