@@ -14,8 +14,13 @@
 // the instructions per logit (6.5 of the 11 that fit into its time at the
 // memory rate). So the pass works in log2 units, where e^(x - M) is one fused
 // multiply-add and one 2^y, with a running reference R = fl(M log2 e): its own
-// rounding is the same for every logit and is taken out of the results again
-// (`residue`). The row is not read a second time for the alternatives: after
+// rounding is the same for every logit of a thread and is taken out of its sums
+// again. It is at most 2^-4 because the pass only holds for maxima within
+// 2^20 of 0 (a rounding of R beyond 2^31 could exceed the exponents of fp32):
+// logits below -2^20, the large negative numbers that stand for masked ones
+// among them, count as -2^20, and parts of rows whose maximum is not within
+// that range are summed again with x - M exact, M being known then. The row is
+// not read a second time for the alternatives: after
 // the pass every thread knows its own maximum, the top-th largest of 32 groups'
 // maxima is a bound that at least `top` logits reach and few others do, and
 // only the threads whose maximum reaches it look at their logits again (a warp
@@ -49,9 +54,9 @@ struct Vec {
   static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);  // NaN if either is
   // The lowest logit that the fast pass tells from minus infinity; a part of a
   // row whose maximum is not well above it takes the exact pass.
-  static constexpr float kLow = Elem<T>::is_bf16 ? -0x1p126f : -65504.f;
+  static constexpr float kLow = Elem<T>::is_bf16 ? -0x1p20f : -65504.f;
   static constexpr uint32_t kNone = Elem<T>::is_bf16 ? 0xff80ff80u : 0xfc00fc00u;  // minus infinity
-  static constexpr uint32_t kLow2 = Elem<T>::is_bf16 ? 0xfe80fe80u : 0xfbfffbffu;
+  static constexpr uint32_t kLow2 = Elem<T>::is_bf16 ? 0xc980c980u : 0xfbfffbffu;
   // -1 in each half that is above the same half of g
   static __device__ __forceinline__ uint32_t above2(uint32_t v, uint32_t g);
   static __device__ __forceinline__ int above(const uint4& v, uint32_t g2, float) {
@@ -102,7 +107,7 @@ __device__ __forceinline__ uint32_t Vec<__half>::above2(uint32_t v, uint32_t g) 
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  static constexpr float kLow = -0x1p126f;
+  static constexpr float kLow = -0x1p20f;
   static constexpr uint32_t kNone = 0xff800000u;
   static __device__ __forceinline__ int above(const uint4& v, uint32_t, float g) {
     return (__uint_as_float(v.x) > g) + (__uint_as_float(v.y) > g) + (__uint_as_float(v.z) > g) + (__uint_as_float(v.w) > g);
@@ -150,21 +155,24 @@ __device__ __forceinline__ unsigned long long key_of(float x, int index) {
   return (static_cast<unsigned long long>(ordered(x)) << 32) | static_cast<uint32_t>(0x7fffffff - index);
 }
 
+// Maxima up to here take the fast pass (see the top).
+constexpr float kHigh = 0x1p20f;
+
 struct Stat {
   float raw;  // maximum, -inf while there is none
-  float r2;  // reference in log2 units, about raw * log2 e
-  float l;  // sum 2^(x log2 e - r2)
-  float s;  // sum 2^(x log2 e - r2) (x log2 e - r2)
+  float ref;  // raw, or a finite number above it where raw is too low for the pass
+  float l;  // sum 2^y, y = (x - ref) log2 e
+  float s;  // sum 2^y y
   int above;  // logits above the given one
 };
 
 __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
   Stat r;
   r.raw = fmaxf(a.raw, b.raw);
-  r.r2 = fmaxf(a.r2, b.r2);
+  r.ref = fmaxf(a.ref, b.ref);
   r.above = a.above + b.above;
   // a side that is far below contributes 0, not 0 * infinity
-  const float da = fmaxf(a.r2 - r.r2, -1e4f), db = fmaxf(b.r2 - r.r2, -1e4f);
+  const float da = fmaxf((a.ref - r.ref) * kLog2e, -1e4f), db = fmaxf((b.ref - r.ref) * kLog2e, -1e4f);
   const float fa = ex2(da), fb = ex2(db);
   r.l = fa * a.l + fb * b.l;
   r.s = fa * fmaf(a.l, da, a.s) + fb * fmaf(b.l, db, b.s);
@@ -174,7 +182,7 @@ __device__ __forceinline__ Stat merge(const Stat& a, const Stat& b) {
 __device__ __forceinline__ Stat shfl_xor(const Stat& a, int o) {
   Stat r;
   r.raw = __shfl_xor_sync(~0u, a.raw, o);
-  r.r2 = __shfl_xor_sync(~0u, a.r2, o);
+  r.ref = __shfl_xor_sync(~0u, a.ref, o);
   r.l = __shfl_xor_sync(~0u, a.l, o);
   r.s = __shfl_xor_sync(~0u, a.s, o);
   r.above = __shfl_xor_sync(~0u, a.above, o);
@@ -258,16 +266,18 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   if constexpr (sizeof(T) == 2) given2 = Elem<T>::pack2(given, given);
 
   // ---- the pass: running maximum, sums, rank
-  Stat st{-INFINITY, Vec<T>::kLow * kLog2e, 0.f, 0.f, 0};
-  uint64_t l2 = 0, s2 = 0, neg2 = pack_f2(-st.r2, -st.r2);  // sums of even and odd elements; -r2 twice
+  Stat st{-INFINITY, 0.f, 0.f, 0.f, 0};
+  float r2 = Vec<T>::kLow * kLog2e;  // the reference, in log2 units
+  uint64_t l2 = 0, s2 = 0, neg2 = pack_f2(-r2, -r2);  // sums of even and odd elements; -r2 twice
   const uint64_t log2e2 = pack_f2(kLog2e, kLog2e);
   auto raise = [&](float x) {
     st.raw = fmaxf(st.raw, x);
-    const float r2 = fmaxf(st.r2, x * kLog2e), d = fmaxf(st.r2 - r2, -1e30f), f = ex2(d);  // 0 * finite
+    const float old = r2;
+    r2 = fmaxf(r2, x * kLog2e);
+    const float d = fmaxf(old - r2, -1e30f), f = ex2(d);  // 0 * finite
     const uint64_t f2 = pack_f2(f, f);
     s2 = fma_f2(f2, fma_f2(l2, pack_f2(d, d), s2), 0);
     l2 = fma_f2(f2, l2, 0);
-    st.r2 = r2;
     neg2 = pack_f2(-r2, -r2);
   };
   auto add2 = [&](float x, float y) {
@@ -300,6 +310,11 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
     st.l = p + q;
     unpack_f2(s2, p, q);
     st.s = p + q;
+    // from the rounded reference to the maximum itself
+    st.ref = fmaxf(st.raw, Vec<T>::kLow);
+    const float d = fmaf(st.ref, kLog2e, -r2), f = ex2(-d);
+    st.s = f * fmaf(-d, st.l, st.s);
+    st.l *= f;
   }
   const bool nan = st.l != st.l;
   s_max[tid] = st.raw == -INFINITY ? 0u : ordered(st.raw);
@@ -332,12 +347,14 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   __syncthreads();
   w = s_all;
   // Where nothing is well above the lowest logit (masked rows), or the maximum
-  // is enormous, the sums again with x - M exact: M is known now.
-  if (!(w.raw > Vec<T>::kLow + 200.f && w.raw < 1e38f) && w.raw < INFINITY && w.l == w.l) {
+  // is enormous, the sums again with x - M exact: M is known now. NaN stays.
+  if (!(w.raw > Vec<T>::kLow + 200.f && w.raw < kHigh)) {
     float l = 0.f, s = 0.f;
     const float m = fmaxf(w.raw, -FLT_MAX);
     auto exact = [&](float x) {
-      const float d = fmaxf((x - m) * kLog2e, -1e30f), e = ex2(d);
+      float d = (x - m) * kLog2e;
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(d) : "f"(-1e30f));
+      const float e = ex2(d);
       l += e;
       s = fmaf(e, d, s);
     };
@@ -356,15 +373,10 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
     }
     if (lane == 0) s_stat[warp].l = l, s_stat[warp].s = s;
     __syncthreads();
-    w.r2 = fminf(fmaxf(m * kLog2e, -3e38f), 3e38f);
+    w.ref = m;
     w.l = w.s = 0.f;
 #pragma unroll
     for (int i = 0; i < kLpWarps; ++i) w.l += s_stat[i].l, w.s += s_stat[i].s;
-    if (fabsf(m) < 1e37f) {  // relative to the rounded reference, as everywhere else
-      const float d = fmaf(m, kLog2e, -w.r2), f = ex2(d);
-      w.s = f * fmaf(w.l, d, w.s);
-      w.l *= f;
-    }
   }
 
   // ---- the largest `top` of this CTA's part of the row
@@ -445,7 +457,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
     cluster_wait();
     const uint32_t dst = mapa(smem_u32(&s_share[rank]), 0);
     if (tid == 0) {
-      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(w.raw), "f"(w.r2), "f"(w.l), "f"(w.s)
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(w.raw), "f"(w.ref), "f"(w.l), "f"(w.s)
                    : "memory");
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 16), "r"(w.above) : "memory");
     }
@@ -461,11 +473,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   }
   const bool empty = w.raw == -INFINITY && w.l == w.l;
   const float log_l = logf(w.l);
-  // what the reference's rounding added to the sums' logarithm
-  const float residue = fabsf(w.raw) < 1e37f ? fmaf(w.raw, kLog2e, -w.r2) * kLn2 : 0.f;
-  auto log_prob = [&](float x) {
-    return empty || (x == -INFINITY && w.l == w.l) ? -INFINITY : (x - w.raw) - (log_l - residue);
-  };
+  auto log_prob = [&](float x) { return empty || (x == -INFINITY && w.l == w.l) ? -INFINITY : (x - w.raw) - log_l; };
   if (tid == 0) {
     a.logprob[t] = log_prob(given);
     if (a.entropy) a.entropy[t] = empty ? 0.f : log_l - kLn2 * (w.s / w.l);

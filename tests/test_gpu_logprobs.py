@@ -152,3 +152,54 @@ def test_refusals(eng):
     p = x.data_ptr()
     assert eng._lib.wp_token_logprobs(eng.handle, p, None, None, None, None, p, 10, p, 4, 2, 100, 0, 1, None) == -1
     assert eng._lib.wp_token_logprobs(None, p, None, None, None, None, p, 100, p, 4, 2, 100, 0, 1, None) == -1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mask", [-1e4, -6e4, -1e6, -1e9, -1e10, -1e12, -1e15, -1e20, -1e30, -1e36, -1e38, -3e38])
+def test_mask_constants(eng, dtype, mask):
+    """Masked logits that hold some large negative number (minus infinity in
+    fp16 where it has no such number): a thread's first vectors, alternate
+    logits, whole parts of a row, all but one, all."""
+    x = logits(7, 40000, dtype)
+    x[0, :64] = mask
+    x[1, 5:] = mask
+    x[2, ::2] = mask
+    x[3, 1000:39000] = mask
+    x[4] = mask
+    x[4, 31234] = 1.5
+    x[5] = mask
+    x[6, 20000:] = mask
+    x[6, :10000] = mask / 3
+    check(eng, x, torch.tensor([100, 3, 1, 39500, 31234, 7, 5]), 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [1e5, 1e6, 2e6, 1e8, 3e9, 1e10, 1e15, 1e30, 1e37, 1e38])
+def test_rows_of_enormous_logits(eng, dtype, size):
+    x = logits(6, 9000, torch.float64)
+    x[0] += size
+    x[1] -= size
+    x[2] *= size / 16
+    x[3, 77] = size
+    x[4, ::3] = size
+    x[4, 1::3] = -size
+    x[5] = size
+    check(eng, x.to(dtype), torch.tensor([100, 3, 1, 77, 1, 7]), 8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rest", [-math.inf, -1e10, 2.0, 3e9, 1e37])
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+def test_nan_and_infinity_among_any_logits(eng, dtype, rest, odd):
+    """One NaN or plus infinity anywhere makes the row NaN, whatever the other
+    logits are; the row beside it is not touched."""
+    x = logits(4, 20000, dtype)
+    want = eng.token_logprobs(x[3:].cuda(), torch.tensor([5]).cuda(), 2)
+    for i, at in enumerate((0, 9999, 19999)):
+        x[i] = rest
+        x[i, at] = odd
+    got = eng.token_logprobs(x.cuda(), torch.tensor([3, 9999, 1, 5]).cuda(), 2)
+    assert bool(got.logprob[:3].isnan().all()) and bool(got.entropy[:3].isnan().all())
+    assert bool(got.top_logprobs[:3].isnan().all())
+    check(eng, x[3:], torch.tensor([5]), 2)
+    assert float(want.logprob[0]) == pytest.approx(float(got.logprob[3]), rel=1e-5)
