@@ -772,7 +772,6 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         unpack_f2(add_f2(sum[0], sum[1]), l0, l1);
         l += l0 + l1;
       }
-      if (m == -INFINITY && l == l) l = 0.f;  // no key seen (the polynomial's smallest value is not 0)
       // ---- the tile's output
       const int64_t at = static_cast<int64_t>(it.s.q0 + token) * a.heads + head;
       T* op = static_cast<T*>(a.out) + at * a.dim;

@@ -234,3 +234,23 @@ def test_which_cta_takes_an_item_does_not_change_results(eng):
     first = eng.prompt_attention(q, k, v, starts(nq), max_q=max(nq))
     for _ in range(10):
         assert torch.equal(eng.prompt_attention(q, k, v, starts(nq), max_q=max(nq)), first)
+
+
+@pytest.mark.parametrize("max_q", [1, 300])
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 3e38), (torch.bfloat16, -1e36), (torch.float16, 65504.0)])
+def test_unseen_values_of_any_size_do_not_reach_a_row(eng, dtype, size, max_q):
+    """The largest finite numbers in V of later tokens, of another sequence and
+    of rows that belong to none: the weight of a key that a row must not see is
+    exactly 0, so every bit of the row stays."""
+    lens = [100, 37, 290]
+    T = sum(lens)
+    q, k, v = (torch.randn(T + 20, 2, 64).to(dtype) for _ in range(3))
+    clean = eng.prompt_attention(q.cuda(), k.cuda(), v.cuda(), starts(lens), max_q=max_q)
+    v[61] = size
+    v[110] = size
+    v[137 + 200, 1] = size
+    v[T:] = size
+    got = eng.prompt_attention(q.cuda(), k.cuda(), v.cuda(), starts(lens), max_q=max_q)
+    for a, b, h in ((0, 61, slice(None)), (100, 110, slice(None)), (137, 337, slice(None)), (337, T, slice(0, 1))):
+        assert torch.equal(got[a:b, h], clean[a:b, h])
+    assert bool(torch.isfinite(got[:T]).all())
