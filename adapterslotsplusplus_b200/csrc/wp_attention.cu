@@ -19,10 +19,10 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "wp_device.cuh"
 #include "wp_internal.h"
+#include "wp_once.h"
 
 namespace wp {
 namespace {
@@ -278,12 +278,12 @@ __global__ void __launch_bounds__(NW * 32) prompt_small_kernel(const __grid_cons
 template <typename T, int D, int NW>
 cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
   using C = SmallCfg<T, D, NW>;
-  static std::atomic<bool> ready{false};
-  if (!ready.load()) {
-    cudaError_t e = cudaFuncSetAttribute(prompt_small_kernel<T, D, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return e;
-    ready.store(true);
-  }
+  static PerDevice ready;
+  if (!ready.get([] {
+        return cudaFuncSetAttribute(prompt_small_kernel<T, D, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) ==
+               cudaSuccess;
+      }))
+    return cudaGetLastError();
   const int group = a.heads / a.kv_heads;
   const int64_t blocks = (static_cast<int64_t>(a.max_q) * group + NW * 16 - 1) / (NW * 16);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(blocks, 1), 4096)), a.kv_heads,
@@ -837,12 +837,12 @@ bool prompt_map(CUtensorMap* m, int dtype, const void* base, int dim, int heads,
 template <typename T, int DP>
 cudaError_t launch_tiles(int dtype, const PromptArgs& a, cudaStream_t stream) {
   using C = PaCfg<DP>;
-  static std::atomic<bool> ready{false};
-  if (!ready.load()) {
-    cudaError_t e = cudaFuncSetAttribute(prompt_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return e;
-    ready.store(true);
-  }
+  static PerDevice ready;
+  if (!ready.get([] {
+        return cudaFuncSetAttribute(prompt_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) ==
+               cudaSuccess;
+      }))
+    return cudaGetLastError();
   const int group = a.heads / a.kv_heads, tpt = kPaRows / group;
   PaMaps maps;
   if (!prompt_map(&maps.q, dtype, a.q, a.dim, a.heads, a.q_tokens, a.q_ts, a.q_hs, group, tpt) ||

@@ -24,10 +24,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <atomic>
-
 #include "wp_device.cuh"
 #include "wp_internal.h"
+#include "wp_once.h"
 
 namespace wp {
 namespace {
@@ -931,18 +930,17 @@ template <typename T, int D, int NT>
 struct Attn {
   // CTAs that one SM holds (0: the kernel cannot run here)
   static int per_sm() {
-    static std::atomic<int> known{-1};
-    int n = known.load();
-    if (n >= 0) return n;
-    using C = AttnCfg<D, NT>;
-    n = 0;
-    if (cudaFuncSetAttribute(kv4_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
-            cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv4_attention_kernel<T, D, NT>, C::THREADS, C::SMEM) !=
-            cudaSuccess)
-      return 0;
-    known.store(n);
-    return n;
+    static PerDevice known;
+    return known.get([] {
+      using C = AttnCfg<D, NT>;
+      int n = 0;
+      if (cudaFuncSetAttribute(kv4_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
+              cudaSuccess ||
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv4_attention_kernel<T, D, NT>, C::THREADS, C::SMEM) !=
+              cudaSuccess)
+        return 0;
+      return n;
+    });
   }
   static int64_t workspace(int num_sms) {
     using C = AttnCfg<D, NT>;
