@@ -64,14 +64,16 @@ class DraftDecoder:
         return (xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + 1e-6)).to(x.dtype)
 
     def forward(self, x: torch.Tensor, seq_len: int, lora: str = "none", pool=None, scale: float = 1.0,
-                torch_lora: Optional[dict] = None, attention: Optional[Callable] = None) -> torch.Tensor:
+                torch_lora: Optional[dict] = None, attention: Optional[Callable] = None,
+                head: bool = True) -> torch.Tensor:
         """x [T, hidden] (T = sequences x seq_len, sequences adapter-sorted).
         lora "pool": pool.add_lora per projection (the segment table must be
         built for this step); "torch": torch_lora = {"ids": [T] adapter ids,
         "A": [p] -> [n_adapters, r, d], "B": [p] -> [n_adapters, o, r]}.
         attention(layer, q, k, v) -> [T, heads, head_dim] on packed q, k, v of
         that shape takes the place of the attention over each sequence's own
-        seq_len tokens (seq_len is then not used)."""
+        seq_len tokens (seq_len is then not used). Logits where the decoder has
+        an LM head; hidden states where it has none, or without `head`."""
         T, H = x.shape
         nh, hd = self.heads, H // self.heads
 
@@ -113,7 +115,7 @@ class DraftDecoder:
             m = (F.silu(g.float()) * u.float()).to(x.dtype).contiguous()
             x = x + proj(base + 6, "down", m, L["down"])
         x = self._rms(x)
-        if self.lm_head is not None:
+        if head and self.lm_head is not None:
             return F.linear(x, self.lm_head)
         return x
 
@@ -169,11 +171,8 @@ class DraftSession:
         return self._hidden(x, attention, lora)
 
     def _hidden(self, x, attention, lora):
-        head, self.model.lm_head = self.model.lm_head, None  # hidden states: score() takes the logits it needs
-        try:
-            return self.model.forward(x, 0, attention=attention, **lora)
-        finally:
-            self.model.lm_head = head
+        # hidden states: score() takes the logits it needs
+        return self.model.forward(x, 0, attention=attention, head=False, **lora)
 
     def score(self, hidden: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
         """Log probability, rank and entropy of a given token per hidden state,
