@@ -116,6 +116,19 @@ __device__ __forceinline__ uint32_t code_of(float d, float step, float inv) {
   return static_cast<uint32_t>(fminf(fmaxf(k, 0.f), 15.f));
 }
 
+// NaN if either is: a row with a NaN gets a NaN zero and scale, so that all its
+// values are NaN and no step after it looks healthy.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Kv4Args a, int per_seq) {
   pdl_wait_prior();
@@ -169,11 +182,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Kv4Args a, int
       }
       float mn = x[0], mx = x[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mn = fminf(mn, x[i]), mx = fmaxf(mx, x[i]);
+      for (int i = 1; i < 16; ++i) mn = min_nan(mn, x[i]), mx = max_nan(mx, x[i]);
 #pragma unroll
       for (int o = PER / 2; o; o >>= 1) {
-        mn = fminf(mn, __shfl_xor_sync(~0u, mn, o));
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+        mn = min_nan(mn, __shfl_xor_sync(~0u, mn, o));
+        mx = max_nan(mx, __shfl_xor_sync(~0u, mx, o));
       }
       const uint32_t pair = Elem<T>::pack2(__fmul_rn(__fsub_rn(mx, mn), 1.0f / 15.0f), mn);
       const float step = Elem<T>::unpack2(pair).x, inv = __frcp_rn(step);

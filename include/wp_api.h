@@ -450,6 +450,7 @@ int wp_prompt_attention(wp_handle* h, void* out, float* lse, const void* q, int6
  * have a (scale, zero) pair in the cache's 16-bit type: zero = min, scale =
  * round16((max - min) * (1/15)), code = rint((x - zero) / scale) clamped to
  * 0..15 (0 where scale is 0), in fp32; a code stands for zero + scale * code.
+ * A row of K or V with a NaN or an infinity is NaN throughout.
  *
  * pages: DEVICE [num_pages][kv_heads][page_size / 16][tile bytes], 16-byte
  * aligned, page_size a multiple of 16, head_dim D = 64 or 128. A tile of 16

@@ -339,3 +339,34 @@ def test_refusals(eng):
     with pytest.raises(WarpPipeError):
         eng._check(lib.wp_kv4_append(h, c.pages.data_ptr(), 1, 24, q.data_ptr(), 8, 8, q.data_ptr(), 8, 8,
                                      b.table.data_ptr(), 2, b.lens.data_ptr(), None, 1, 1, 2, 64, 1, None))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_nan_and_infinity_stay_in_the_cache(eng, dtype, dim):
+    """A NaN or an infinity in a row of K or V makes that row NaN (its scale or
+    zero is none or infinite), for read and for the queries that see it, and
+    nothing else."""
+    clean = Batch(eng, [70, 20], 2, dim, dtype).append_all()
+    b = Batch(eng, [70, 20], 2, dim, dtype)
+    b.k[0][66, 0, 3] = math.nan
+    b.v[0][67, 1, dim - 1] = math.nan
+    b.k[1][19, 0, 9] = -math.nan
+    b.v[1][3, 1, 0] = math.inf
+    b.append_all()
+    k, v = b.cache.read(b.table, b.lens, starts([70, 20]), 90)
+    for got, x in ((k, b.k), (v, b.v)):
+        want = torch.cat([kv4_values(y) for y in x]).to(dtype)
+        assert torch.equal(got.cpu().isnan(), want.isnan())
+        assert torch.equal(got.cpu().nan_to_num(7.0), want.nan_to_num(7.0))
+    assert bool(k[66, 0].isnan().all()) and bool(v[67, 1].isnan().all()) and bool(k[89, 0].isnan().all())
+    q = torch.randn(9, 4, dim, device="cuda").to(dtype)
+    got = b.cache.attention(q, b.table, b.lens, starts([6, 3]), 6)
+    want = clean.cache.attention(q, clean.table, clean.lens, starts([6, 3]), 6)
+    bad = torch.zeros(9, 4, dtype=torch.bool)
+    bad[2:6, :2] = True  # token 66 and later see K's NaN of the first kv head
+    bad[3:6, 2:] = True  # token 67 and later V's of the second
+    bad[8, :2] = True
+    bad[6:, 2:] = True
+    assert torch.equal(got.cpu().isnan(), bad[..., None].expand_as(got))
+    assert torch.equal(got.cpu()[~bad], want.cpu()[~bad])
