@@ -5,9 +5,12 @@
 //   p_ij = 2^((scale q[i, h] . k[j, h / G] - m_i) log2 e),  j <= i + nk - nq
 // per sequence of nq query and nk key tokens (bottom-right causal: a chunk of a
 // prompt follows its context). Scores, maxima, sums and outputs are fp32; the
-// weights p are rounded to the inputs' 16-bit type for the second product (at
-// most 1, so the rounding is relative, as the output's own is) while their sum
-// is taken before the rounding. A row that sees no key is 0.
+// weights p are rounded to the inputs' 16-bit type for the second product
+// while their sum is taken before the rounding. The rounding is relative, as
+// the output's own is: bf16 has fp32's exponents, and in fp16 weights and sum
+// have a power of two as a factor (`kWeightUp`) that uses its range up to 2^15:
+// weights down to 2^-22 of the row's largest are normal numbers, and those down
+// to 2^-33 count. A row that sees no key is 0.
 //
 // Query rows of one kv head are packed: row r of a sequence's (kv head) is
 // token r / G, head r % G of the group, so grouped heads share every K and V
@@ -30,6 +33,12 @@ namespace {
 struct PromptSeq {
   int q0, nq, k0, nk;
 };
+
+// log2 of what a weight of 2^0 is multiplied by, for weights up to 2^lazy.
+template <typename T>
+__device__ constexpr float weight_up(float lazy) {
+  return Elem<T>::is_bf16 ? 0.f : 15.f - lazy;
+}
 
 // A sequence's rows, forced into the packed tensors (offsets outside them
 // raise the error bit).
@@ -114,6 +123,7 @@ __global__ void __launch_bounds__(NW * 32) prompt_small_kernel(const __grid_cons
   using C = SmallCfg<T, D, NW>;
   using E = Elem<T>;
   constexpr int BN = C::BN, LD = C::LD, KS = D / 16;
+  constexpr float kWeightUp = weight_up<T>(0.f);
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.y, group = a.heads / a.kv_heads;
@@ -213,6 +223,7 @@ __global__ void __launch_bounds__(NW * 32) prompt_small_kernel(const __grid_cons
         const float mn = fmaxf(m[i], top[i]);
         base[i] = mn == -INFINITY ? 0.f : mn;
         const float f = ex2(m[i] - base[i]);
+        base[i] -= kWeightUp;
         m[i] = mn;
         l[i] *= f;
 #pragma unroll
@@ -260,7 +271,7 @@ __global__ void __launch_bounds__(NW * 32) prompt_small_kernel(const __grid_cons
         bad[i] |= !(fabsf(x) <= 3e38f) || !(fabsf(y) <= 3e38f);
         if (r < rows && d < chunks) *reinterpret_cast<uint32_t*>(op + d * 8) = E::pack2(x, y);
       }
-      if (a.lse && c == 0 && r < rows) a.lse[at] = l[i] == 0.f ? -INFINITY : (m[i] + __log2f(l[i])) * kLn2;
+      if (a.lse && c == 0 && r < rows) a.lse[at] = l[i] == 0.f ? -INFINITY : (m[i] + (__log2f(l[i]) - kWeightUp)) * kLn2;
       bad[i] &= r < rows;
     }
 #pragma unroll
@@ -314,8 +325,8 @@ cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
 // before j. P V starts on the first 64 keys' weights.
 //
 // The running maximum is only raised when a row's grows by more than 8 (in
-// log2 units): weights then reach 2^8 at most, which costs fp16 and bf16
-// nothing, and O is rescaled in a few blocks at the start instead of in most.
+// log2 units; 7 in fp16): weights then reach 2^8 at most (2^15 with fp16's
+// factor), and O is rescaled in a few blocks at the start instead of in most.
 //
 // The grid has a CTA per item, in the order (sequence, pairs from the last one,
 // kv head), so long items come first within a sequence. A resident CTA that
@@ -336,7 +347,8 @@ constexpr int kPaProd = 8;
 constexpr int kPaMma = 9;
 constexpr int kPaRows = 128;  // rows of a tile
 constexpr int kPaKeys = 128;  // keys of a block
-constexpr float kPaLazy = 8.f;
+template <typename T>
+constexpr float kPaLazy = Elem<T>::is_bf16 ? 8.f : 7.f;
 // Of 8 pairs of weights, those that take the FMA pipe instead of the special-
 // function unit. 32 query / 8 kv heads of 128, bf16, for 1, 2 and 3: 4 x 2048
 // tokens 158, 151 and 152 us, 64 x 100-400 tokens 126, 123 and 126, 1 x 8192
@@ -376,6 +388,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   using C = PaCfg<DP>;
   using E = Elem<T>;
   constexpr int S = C::S;
+  constexpr float kWeightUp = weight_up<T>(kPaLazy<T>);
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem);  // [S]
   uint64_t* kv_empty = kv_full + 8;  // [S]
@@ -722,7 +735,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         row_max(x[2], 64);
         row_max(x[3], 96);
         const float top = max3(max3(t[0], t[1], t[2]), t[3], -INFINITY);
-        if (__any_sync(~0u, (top - m) * sc > kPaLazy || (m == -INFINITY && top > m))) {
+        if (__any_sync(~0u, (top - m) * sc > kPaLazy<T> || (m == -INFINITY && top > m))) {
           const float mn = fmaxf(m, top);
           const float f = m == -INFINITY ? 0.f : ex2((m - mn) * sc);
           m = mn;
@@ -740,7 +753,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           }
         }
         if (!(top < INFINITY)) l = NAN;  // NaN and infinite scores: the polynomial would lose them
-        const float off = m == -INFINITY ? 0.f : -m * sc;
+        const float off = m == -INFINITY ? 0.f : fmaf(-m, sc, kWeightUp);
         const uint64_t sc2 = pack_f2(sc, sc), off2 = pack_f2(off, off);
         uint64_t sum[2] = {0, 0};
         // 64 keys at a time, so that the second product starts on the first half
@@ -810,7 +823,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 #pragma unroll 1
         for (int d = 0; d < a.dim; d += 8) *reinterpret_cast<uint4*>(op + d) = make_uint4(0, 0, 0, 0);
       }
-      if (a.lse && live) a.lse[at] = l == 0.f ? -INFINITY : (m * sc + __log2f(l)) * kLn2;
+      if (a.lse && live) a.lse[at] = l == 0.f ? -INFINITY : (m * sc + (__log2f(l) - kWeightUp)) * kLn2;
       for (unsigned todo = __ballot_sync(~0u, odd && live); todo; todo &= todo - 1) {
         const int r = (warp & 3) * 32 + __ffs(todo) - 1;
         prompt_row<T>(a, it.s, first + r / group, it.kvh * group + r % group);

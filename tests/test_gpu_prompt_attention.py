@@ -254,3 +254,28 @@ def test_unseen_values_of_any_size_do_not_reach_a_row(eng, dtype, size, max_q):
     for a, b, h in ((0, 61, slice(None)), (100, 110, slice(None)), (137, 337, slice(None)), (337, T, slice(0, 1))):
         assert torch.equal(got[a:b, h], clean[a:b, h])
     assert bool(torch.isfinite(got[:T]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("empty", [0, 70])
+def test_many_small_weights_beside_a_large_one(eng, dtype, empty):
+    """60000 keys of weight e^-18 (2^-26 of the first key's, below what fp16
+    holds) whose sum counts: out = n e^-18 / (1 + n e^-18). All V are of one
+    sign, so a weight's relative error moves the result by as much: u / 2 for
+    the weights, u / 2 for the result, 2^-10 for the scores (see the top); and
+    half a step of the smallest 16-bit weight, 2^-33 of the largest, per key.
+    (With 70 empty sequences beside it the call takes the warp-level kernel.)"""
+    n = 60000
+    q = torch.ones(3, 1, 64, dtype=dtype)
+    k = torch.zeros(n, 1, 64, dtype=dtype)
+    k[0] = 1
+    v = torch.ones(n, 1, 64, dtype=dtype)
+    v[0] = 0
+    out, lse = eng.prompt_attention(q.cuda(), k.cuda(), v.cuda(), starts([3] + [0] * empty), starts([n] + [0] * empty), 3,
+                                    18 / 64, True)
+    tail = torch.tensor([n - 3, n - 2, n - 1], dtype=torch.float64) * math.exp(-18)
+    ref = (tail / (1 + tail))[:, None, None]
+    u = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    err = (out.double().cpu() - ref).abs()
+    assert float((err - (u + 2.0 ** -10) * ref).max()) <= n * 2.0 ** -33, float(err.max())
+    assert float((lse.double().cpu() - (18 + torch.log1p(tail))[:, None]).abs().max()) <= 2.0 ** -10
