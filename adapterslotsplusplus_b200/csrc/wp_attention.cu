@@ -54,38 +54,65 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptArgs& a, int b) {
   return PromptSeq{q0, q1 - q0, k0, k1 - k0};
 }
 
-// One row by one warp, over its visible keys only, element by element. The
-// tiled kernels multiply the weight 0 of a key that a row must not see with
-// that key's V, which is NaN where V is not finite; rows whose result is not
-// finite come here, so only a row's own keys decide what it is.
+// One row by one warp, over its visible keys only. The tiled kernels multiply
+// the weight 0 of a key that a row must not see with that key's V, which is NaN
+// where V is not finite; rows whose result is not finite come here, so only a
+// row's own keys decide what it is. 32 keys at a time: a lane has the score of
+// one of them, then four dimensions of the output. `beat` (shared memory, or
+// null) is raised every 1024 keys, for those who wait meanwhile. The caller has
+// passed a __syncwarp since the row's first stores.
 template <typename T>
-__device__ __forceinline__ void prompt_row(const PromptArgs& a, const PromptSeq& s, int token, int head) {
+__device__ __forceinline__ void prompt_row(const PromptArgs& a, const PromptSeq& s, int token, int head, int* beat) {
   const int lane = threadIdx.x & 31, d0 = lane * 4, kvh = head / (a.heads / a.kv_heads);
   const bool on = d0 < a.dim;
-  auto load = [&](const T* p, float (&x)[4]) {
-    const uint2 w = on ? __ldg(reinterpret_cast<const uint2*>(p + d0)) : make_uint2(0, 0);
-    const float2 f = Elem<T>::unpack2(w.x), g = Elem<T>::unpack2(w.y);
-    x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
-  };
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  load(static_cast<const T*>(a.q) + static_cast<int64_t>(s.q0 + token) * a.q_ts + head * a.q_hs, q);
+  const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(s.q0 + token) * a.q_ts + head * a.q_hs;
+  const T* k = static_cast<const T*>(a.k) + static_cast<int64_t>(s.k0) * a.k_ts + kvh * a.k_hs;
+  const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(s.k0) * a.v_ts + kvh * a.v_hs + (on ? d0 : 0);
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
   const int end = min(token + s.nk - s.nq + 1, s.nk);
 #pragma unroll 1
-  for (int j = 0; j < end; ++j) {
-    float k[4], v[4];
-    load(static_cast<const T*>(a.k) + static_cast<int64_t>(s.k0 + j) * a.k_ts + kvh * a.k_hs, k);
-    load(static_cast<const T*>(a.v) + static_cast<int64_t>(s.k0 + j) * a.v_ts + kvh * a.v_hs, v);
-    float x = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+  for (int j0 = 0; j0 < end; j0 += 32) {
+    if (beat && lane == 0 && (j0 & 1023) == 0) atomicAdd(beat, 1);
+    float x = -INFINITY;
+    if (j0 + lane < end) {
+      const T* kr = k + (j0 + lane) * a.k_ts;
+      x = 0.f;
+#pragma unroll 2
+      for (int d = 0; d < a.dim; d += 8) {
+        const uint4 kw = __ldg(reinterpret_cast<const uint4*>(kr + d)), qw = __ldg(reinterpret_cast<const uint4*>(q + d));
+        const uint32_t ku[4] = {kw.x, kw.y, kw.z, kw.w}, qu[4] = {qw.x, qw.y, qw.z, qw.w};
 #pragma unroll
-    for (int off = 16; off; off >>= 1) x += __shfl_xor_sync(~0u, x, off);
-    x *= a.scale * kLog2e;
-    const float mn = x > m ? x : m, base = mn == -INFINITY ? 0.f : mn;
-    const float f = ex2(m - base), p = ex2(x - base);
-    m = mn;
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = Elem<T>::unpack2(ku[i]), g = Elem<T>::unpack2(qu[i]);
+          x = fmaf(f.x, g.x, x);
+          x = fmaf(f.y, g.y, x);
+        }
+      }
+      x *= a.scale * kLog2e;
+    }
+    float top = x;
+#pragma unroll
+    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, off));
+    top = fmaxf(m, top);
+    const float base = top == -INFINITY ? 0.f : top, f = ex2(m - base), p = ex2(x - base);
+    m = top;
     l = l * f + p;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * f + p * v[i];
+    for (int i = 0; i < 4; ++i) o[i] *= f;
+    const int n = min(end - j0, 32);
+#pragma unroll 8
+    for (int t = 0; t < n; ++t) {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(v + (j0 + t) * a.v_ts));
+      const float2 f0 = Elem<T>::unpack2(w.x), f1 = Elem<T>::unpack2(w.y);
+      const float pt = __shfl_sync(~0u, p, t);
+      o[0] = fmaf(pt, f0.x, o[0]);
+      o[1] = fmaf(pt, f0.y, o[1]);
+      o[2] = fmaf(pt, f1.x, o[2]);
+      o[3] = fmaf(pt, f1.y, o[3]);
+    }
   }
+#pragma unroll
+  for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(~0u, l, off);
   const int64_t at = static_cast<int64_t>(s.q0 + token) * a.heads + head;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (on)
@@ -272,14 +299,15 @@ __global__ void __launch_bounds__(NW * 32) prompt_small_kernel(const __grid_cons
         if (r < rows && d < chunks) *reinterpret_cast<uint32_t*>(op + d * 8) = E::pack2(x, y);
       }
       if (a.lse && c == 0 && r < rows) a.lse[at] = l[i] == 0.f ? -INFINITY : (m[i] + (__log2f(l[i]) - kWeightUp)) * kLn2;
-      bad[i] &= r < rows;
+      bad[i] &= r < rows && l[i] == l[i];  // a NaN among the row's own scores: all of it is NaN
     }
+    __syncwarp();  // a row's first stores come from other lanes
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       for (unsigned todo = __ballot_sync(~0u, bad[i]); todo;) {
         const int lead = __ffs(todo) - 1, r = r0 + warp * 16 + (lead >> 2) + 8 * i;
         todo &= ~(0xfu << (lead & ~3));
-        prompt_row<T>(a, s, r / group, kvh * group + r % group);
+        prompt_row<T>(a, s, r / group, kvh * group + r % group, nullptr);
       }
     __syncthreads();  // the next block's loads overwrite Q and the tiles
     rb += gridDim.x;
@@ -401,6 +429,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   uint64_t* o_free = kv_full + 30;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(kv_full + 32);
   volatile int* s_bad = reinterpret_cast<volatile int*>(kv_full + 33);
+  int* s_beat = reinterpret_cast<int*>(kv_full + 33) + 1;  // grows while rows are computed again
   uint64_t* next_full = kv_full + 40;  // *s_item is the next item
   uint64_t* next_empty = kv_full + 41;
   uint64_t* taken = kv_full + 42;  // a cancellation's answer is there
@@ -434,6 +463,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     mbar_init(next_empty, kPaWarps - 1);
     mbar_init(taken, 1);
     *s_bad = 0;
+    *s_beat = 0;
     fence_mbar_init();
   }
   if (warp == 0) tmem_alloc(s_tmem, 512);
@@ -465,9 +495,24 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   s_sum[tid] = before + incl - mine;
   __syncthreads();
 
+  // Waits of a warp and of one lane. Rows that are computed again (prompt_row)
+  // take as long as their sequence is long, so a wait goes on where its limit
+  // runs out while some row has come further since the last time.
+  auto wait_warp = [&](uint32_t bar, uint32_t parity) { return mbar_wait_warp(bar, parity, a.err, s_beat); };
+  auto wait_lane = [&](uint64_t* bar, uint32_t parity) {
+    for (int seen = 0; !mbar_wait_bounded(bar, parity, nullptr);) {
+      const int now = *const_cast<volatile int*>(s_beat);
+      if (now == seen) {
+        if (a.err) atomicOr(a.err, kErrWaitTimeout);
+        return false;
+      }
+      seen = now;
+    }
+    return true;
+  };
   // Waits for the CTA's n-th item, a whole warp together; false past the last one.
   auto item = [&](int n, PaItem& it) {
-    if (!mbar_wait_warp(smem_u32(next_full), n & 1, a.err)) {
+    if (!wait_warp(smem_u32(next_full), n & 1)) {
       *s_bad = 1;
       return false;
     }
@@ -495,7 +540,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         if (lane == 0 && !*s_bad) {
           for (int i = 0; i < 2; ++i) {
             if (it.n[i] <= 0) continue;
-            if (qn[i] > 0 && !mbar_wait_bounded(&q_empty[i], (qn[i] - 1) & 1, a.err)) *s_bad = 1;
+            if (qn[i] > 0 && !wait_lane(&q_empty[i], (qn[i] - 1) & 1)) *s_bad = 1;
             ++qn[i];
             mbar_arrive_expect_tx(&q_full[i], q_bytes);
             for (int sl = 0; sl < C::SL; ++sl)
@@ -505,7 +550,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 #pragma unroll 1
           for (int j = 0; j < 2 * blocks && !*s_bad; ++j, ++u) {
             const int st = u % S;
-            if (u >= S && !mbar_wait_bounded(&kv_empty[st], ((u / S) - 1) & 1, a.err)) {
+            if (u >= S && !wait_lane(&kv_empty[st], ((u / S) - 1) & 1)) {
               *s_bad = 1;
               break;
             }
@@ -542,7 +587,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       uint32_t st = 0, ph = 0;  // ring position of the next block
       uint32_t q_par = 0, p_par = 0, o_par = 1, t_par = i ? 0 : 1;
       bool ok = true;
-      auto wait = [&](uint32_t at, uint32_t parity) { ok = ok && mbar_wait_warp(at, parity, a.err); };
+      auto wait = [&](uint32_t at, uint32_t parity) { ok = ok && wait_warp(at, parity); };
       auto next = [&] {
         if (++st == S) {
           st = 0;
@@ -637,7 +682,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 #pragma unroll 1
       for (int n = 0, x = blockIdx.x; x >= 0; ++n) {
         if (lane == 0) {
-          bool ok = n == 0 || mbar_wait_bounded(next_empty, (n - 1) & 1, a.err);
+          bool ok = n == 0 || wait_lane(next_empty, (n - 1) & 1);
           for (bool more = n > 0; ok && (more || x >= total); more = false) {
             mbar_arrive_expect_tx(taken, 16);
             cancel_cta(s_answer, taken);
@@ -703,7 +748,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int j = 0; j < blocks; ++j) {
-        if (!mbar_wait_warp(smem_u32(&s_full[i]), sn++ & 1, a.err)) {
+        if (!wait_warp(smem_u32(&s_full[i]), sn++ & 1)) {
           *s_bad = 1;
           break;
         }
@@ -790,7 +835,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       T* op = static_cast<T*>(a.out) + at * a.dim;
       bool odd = false;
       if (blocks > 0) {
-        if (__any_sync(~0u, *s_bad) || !mbar_wait_warp(smem_u32(&o_full[i]), on++ & 1, a.err)) {
+        if (__any_sync(~0u, *s_bad) || !wait_warp(smem_u32(&o_full[i]), on++ & 1)) {
           *s_bad = 1;
           break;
         }
@@ -824,9 +869,11 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         for (int d = 0; d < a.dim; d += 8) *reinterpret_cast<uint4*>(op + d) = make_uint4(0, 0, 0, 0);
       }
       if (a.lse && live) a.lse[at] = l == 0.f ? -INFINITY : (m * sc + (__log2f(l) - kWeightUp)) * kLn2;
-      for (unsigned todo = __ballot_sync(~0u, odd && live); todo; todo &= todo - 1) {
+      // (where l is NaN, one of the row's own scores is, and all of it is NaN)
+      __syncwarp();  // a row's first stores come from another lane
+      for (unsigned todo = __ballot_sync(~0u, odd && live && l == l); todo; todo &= todo - 1) {
         const int r = (warp & 3) * 32 + __ffs(todo) - 1;
-        prompt_row<T>(a, it.s, first + r / group, it.kvh * group + r % group);
+        prompt_row<T>(a, it.s, first + r / group, it.kvh * group + r % group, s_beat);
       }
     }
   }

@@ -279,3 +279,24 @@ def test_many_small_weights_beside_a_large_one(eng, dtype, empty):
     err = (out.double().cpu() - ref).abs()
     assert float((err - (u + 2.0 ** -10) * ref).max()) <= n * 2.0 ** -33, float(err.max())
     assert float((lse.double().cpu() - (18 + torch.log1p(tail))[:, None]).abs().max()) <= 2.0 ** -10
+
+
+def test_rows_computed_again_hold_nobody_up(eng):
+    """An infinity near the start of 400000 keys sends every row of the long
+    sequence to the kernel's exact path, over a second of it in each warp, while
+    other items of the same CTA wait. All of them come out: the rows that see
+    the infinity, their other dimensions, and the sequence beside it, whose bits
+    stay. Bound: at the top, once for each side."""
+    nq, nk = [10240, 300], [400000, 300]
+    q, k, v = (torch.randn(n, 4, 64, device="cuda", dtype=torch.bfloat16) for n in (sum(nq), sum(nk), sum(nk)))
+    clean = eng.prompt_attention(q, k, v, starts(nq), starts(nk), 10240)
+    v[5, :, 3] = math.inf
+    got = eng.prompt_attention(q, k, v, starts(nq), starts(nk), 10240)
+    assert eng.device_error(clear=True) == 0
+    assert torch.equal(got[10240:], clean[10240:])
+    assert bool((got[:10240, :, 3] == math.inf).all())
+    rest = [d for d in range(64) if d != 3]
+    a, b = got[:10240, :, rest].float(), clean[:10240, :, rest].float()
+    u = 2.0 ** -8
+    big = float(v[:, :, rest].float().abs().max())
+    assert bool(((a - b).abs() <= 2 * (u / 2 * b.abs() + (u / 2 + 2.0 ** -10) * big)).all())
