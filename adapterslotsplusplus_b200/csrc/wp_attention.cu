@@ -433,6 +433,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   uint64_t* next_full = kv_full + 40;  // *s_item is the next item
   uint64_t* next_empty = kv_full + 41;
   uint64_t* taken = kv_full + 42;  // a cancellation's answer is there
+  uint64_t* drained = kv_full + 50;  // an issuer's products have ended (where a wait ran out)
   uint4* s_answer = reinterpret_cast<uint4*>(kv_full + 44);
   PaItem* s_item = reinterpret_cast<PaItem*>(kv_full + 46);
   int* s_warp = reinterpret_cast<int*>(kv_full + 34);  // [kPaWarps]
@@ -456,6 +457,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       mbar_init(&p_full[2 * i], 4);
       mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&turn[i], 1);
+      mbar_init(&drained[i], 1);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_free[i], 4);
     }
@@ -563,8 +565,11 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         if (lane == 0) mbar_arrive(next_empty);
         __syncwarp();
       }
-      if (lane == 0 && *s_bad)  // a wait ran out: let the copies in flight land before the CTA leaves
+      if (lane == 0) {  // copies in flight land before the CTA leaves, also where a wait ran out
         for (int i = max(u - S, 0); i < u; ++i) mbar_wait_bounded(&kv_full[i % S], (i / S) & 1, a.err);
+        for (int i = 0; i < 2; ++i)
+          if (qn[i] > 0) mbar_wait_bounded(&q_full[i], (qn[i] - 1) & 1, a.err);
+      }
     } else if (warp < kPaMma + 2) {
       // ==================== MMA issuer of tile i ============================
       // Runs converged and issues from one lane; descriptors are sums of
@@ -667,12 +672,13 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           __syncwarp();
         }
       }
-      if (!ok) {
+      if (!ok || *s_bad) {
         // a wait ran out: stop the others, and let the products in flight end
         // before TMEM is freed
         *s_bad = 1;
-        if (elect_one()) umma_commit_at(bar(o_full) + 8 * i);
-        mbar_wait_bounded(o_full + i, 0, a.err, 1000000ull);
+        __syncwarp();
+        if (elect_one()) umma_commit_at(bar(drained) + 8 * i);
+        mbar_wait_bounded(drained + i, 0, a.err, 1000000ull);
       }
     } else {
       // ============================ items ====================================
