@@ -556,8 +556,10 @@ __global__ void __launch_bounds__(AttnCfg<D, NT>::THREADS, 1) kv4_attention_kern
     }
 
     const int st = it % C::S;
-    if (issued < count) issue();
-    if (ok) ok = mbar_wait_bounded(&bar[st], (it / C::S) & 1, a.err);
+    // once a wait has run out (in any lane: the whole warp goes on alike),
+    // nothing is loaded any more
+    if (ok && issued < count) issue();
+    if (ok) ok = __all_sync(~0u, mbar_wait_bounded(&bar[st], (it / C::S) & 1, a.err));
     const uint8_t* sp = ring + st * C::STAGE;
     const int left = con.s.len - con.t * kKv4Chunk;  // tokens from here on
     if (ok && left > 0) {
@@ -832,6 +834,8 @@ __global__ void __launch_bounds__(AttnCfg<D, NT>::THREADS, 1) kv4_attention_kern
     }
     if (it + 1 < count) con.next(a, group, C::ROWS);
   }
+  if (!ok)  // let the copies in flight land before the CTA leaves
+    for (int i = max(issued - C::S, 0); i < issued; ++i) mbar_wait_bounded(&bar[i % C::S], (i / C::S) & 1, a.err);
 }
 
 // Adds the partial rows of segments that several warps shared, in warp order.
