@@ -50,18 +50,19 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def _index(t: torch.Tensor, what: str, dims: int) -> torch.Tensor:
-    """An index tensor as the kernels take it: int32, CUDA, contiguous."""
-    if not t.is_cuda or t.dtype != torch.int32 or t.dim() != dims:
-        raise RuntimeError(f"{what} must be a {dims}-d int32 CUDA tensor")
+def _index(t: torch.Tensor, what: str, dims: int, device: torch.device) -> torch.Tensor:
+    """An index tensor as the kernels take it: int32, on the engine's device,
+    contiguous."""
+    if t.get_device() != device.index or t.dtype != torch.int32 or t.dim() != dims:
+        raise RuntimeError(f"{what} must be a {dims}-d int32 tensor on {device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _packed_rows(t: torch.Tensor, what: str) -> torch.Tensor:
+def _packed_rows(t: torch.Tensor, what: str, device: torch.device) -> torch.Tensor:
     """[tokens, heads, dim] with rows that 16-byte loads can take, copied only
     when the strides or the address do not allow them."""
-    if not t.is_cuda:
-        raise RuntimeError(f"{what} must be a CUDA tensor")
+    if t.get_device() != device.index:
+        raise RuntimeError(f"{what} must be a tensor on {device}")
     tokens, heads, dim = t.stride()
     if dim != 1 or tokens % 8 or heads % 8 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format)
@@ -377,7 +378,8 @@ class WarpPipeEngine:
         dim ** -0.5; max_q, the most query tokens of one sequence, chooses the
         kernel only. Returns out like q (contiguous), and the softmax's log
         denominators [tokens, heads] in fp32 with return_lse. A row that sees
-        no key is 0 (lse -inf)."""
+        no key is 0 (lse -inf); rows outside every sequence's offsets are not
+        written."""
         if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape != v.shape:
             raise RuntimeError("prompt_attention: q must be [tokens, heads, dim], k and v [key tokens, kv_heads, dim]")
         dt = _dtype_code(q, "prompt_attention: q/k/v")
@@ -387,11 +389,12 @@ class WarpPipeEngine:
         keys, kv_heads, k_dim = k.shape
         if k_dim != dim or kv_heads == 0 or heads == 0 or heads % kv_heads:
             raise RuntimeError(f"prompt_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not go together")
-        q = _packed_rows(q, "prompt_attention: q")
-        k = _packed_rows(k, "prompt_attention: k")
-        v = _packed_rows(v, "prompt_attention: v")
-        cu_q = _index(cu_q, "prompt_attention: cu_q", 1)
-        cu_k = cu_q if cu_k is None else _index(cu_k, "prompt_attention: cu_k", 1)
+        dev = self.device
+        q = _packed_rows(q, "prompt_attention: q", dev)
+        k = _packed_rows(k, "prompt_attention: k", dev)
+        v = _packed_rows(v, "prompt_attention: v", dev)
+        cu_q = _index(cu_q, "prompt_attention: cu_q", 1, dev)
+        cu_k = cu_q if cu_k is None else _index(cu_k, "prompt_attention: cu_k", 1, dev)
         n = cu_q.numel() - 1
         if n < 0 or cu_k.numel() != n + 1:
             raise RuntimeError("prompt_attention: cu_q and cu_k must have one entry more than there are sequences")
@@ -412,8 +415,9 @@ class WarpPipeEngine:
         `top` (at most 32) largest alternatives, equal logits by ascending id.
         tokens [rows] int32 or int64; one outside the vocabulary has log
         probability -inf."""
-        if not (logits.is_cuda and tokens.is_cuda):
-            raise RuntimeError("token_logprobs: logits/tokens must be CUDA tensors")
+        dev = self.device
+        if logits.get_device() != dev.index or tokens.get_device() != dev.index:
+            raise RuntimeError(f"token_logprobs: logits/tokens must be tensors on {dev}")
         code = _lib.WP_DTYPE_F32 if logits.dtype == torch.float32 else _dtype_code(logits, "token_logprobs: logits")
         if tokens.dtype not in (torch.int32, torch.int64):
             raise RuntimeError("token_logprobs: tokens must be int32 or int64")
@@ -429,7 +433,6 @@ class WarpPipeEngine:
             ld = vocab
         if not tokens.is_contiguous():
             tokens = tokens.contiguous()
-        dev = logits.device
         # one allocation: log probabilities, entropies, the alternatives' log
         # probabilities; ranks, the alternatives' ids
         buf = torch.empty(rows * (3 + 2 * top), dtype=torch.float32, device=dev)

@@ -46,8 +46,9 @@ class KvCache4:
                                    "a multiple of 16")
             pages = torch.zeros(num_pages, kv_heads, page_size // self.TILE, self._lib.wp_kv4_tile_bytes(head_dim),
                                 dtype=torch.uint8, device=engine.device)
-        if pages.dtype != torch.uint8 or pages.dim() != 4 or not pages.is_cuda or not pages.is_contiguous():
-            raise RuntimeError("KvCache4: pages must be a contiguous 4-d uint8 CUDA tensor")
+        if (pages.dtype != torch.uint8 or pages.dim() != 4 or pages.get_device() != engine.device.index
+                or not pages.is_contiguous()):
+            raise RuntimeError(f"KvCache4: pages must be a contiguous 4-d uint8 tensor on {engine.device}")
         if pages.size(3) not in (16 * 64 + 128, 16 * 128 + 128):
             raise RuntimeError("KvCache4: pages.size(3) must be 16 * head_dim + 128 with head_dim 64 or 128")
         self.pages = pages
@@ -59,8 +60,9 @@ class KvCache4:
         self._work_bytes: Dict[Tuple[int, int], int] = {}  # (heads, max_q) -> attention's workspace
 
     def _place(self, table, lens, cu, tokens: int, what: str) -> Tuple:
-        table = _index(table, f"{what}: table", 2)
-        lens = _index(lens, f"{what}: lens", 1)
+        dev = self.engine.device
+        table = _index(table, f"{what}: table", 2, dev)
+        lens = _index(lens, f"{what}: lens", 1, dev)
         n = lens.numel()
         if table.size(0) != n:
             raise RuntimeError(f"{what}: table and lens must have one row per sequence")
@@ -68,7 +70,7 @@ class KvCache4:
             if tokens != n:
                 raise RuntimeError(f"{what}: without cu every sequence has one token")
         else:
-            cu = _index(cu, f"{what}: cu", 1)
+            cu = _index(cu, f"{what}: cu", 1, dev)
             if cu.numel() != n + 1:
                 raise RuntimeError(f"{what}: cu must have one entry more than there are sequences")
         return table, lens, cu, n
@@ -79,7 +81,7 @@ class KvCache4:
             raise RuntimeError(f"{what} must be [tokens, {heads or 'heads'}, {self.head_dim}]")
         if t.dtype != self.dtype:
             raise RuntimeError(f"{what} must be of the cache's dtype {self.dtype}, got {t.dtype}")
-        return _packed_rows(t, what)
+        return _packed_rows(t, what, self.engine.device)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, table, lens, cu=None) -> None:
         """Stores k and v [tokens, kv_heads, head_dim] as the last tokens of
@@ -101,7 +103,8 @@ class KvCache4:
     def read(self, table, lens, cu=None, tokens: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """The values that the last cu[b + 1] - cu[b] tokens of each sequence
         stand for, as packed k and v [tokens, kv_heads, head_dim]; tokens:
-        their total, the length of the packed tensors (needed with cu)."""
+        their total, the length of the packed tensors (needed with cu). Rows
+        past the last sequence's, where tokens is more, are not written."""
         if tokens is None:
             if cu is not None:
                 raise RuntimeError("read: tokens (the total, cu[-1]) is needed with cu")
@@ -125,7 +128,8 @@ class KvCache4:
         to head_dim ** -0.5; max_q, the most query tokens of one sequence,
         chooses the kernel only. Returns out like q (contiguous), and the
         softmax's log denominators [tokens, heads] in fp32 with return_lse. A
-        row that sees nothing is 0 (lse -inf)."""
+        row that sees nothing is 0 (lse -inf); rows outside every sequence's
+        offsets are not written."""
         q = self._rows(q, 0, "attention: q")
         tokens, heads, _ = q.shape
         if heads == 0 or heads % self.kv_heads:

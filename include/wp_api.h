@@ -440,7 +440,7 @@ int wp_add_lora_row_parallel(wp_handle* h, void* y, const void* x, const void* w
  * sees no key is 0 with lse -inf; what a row must not see does not reach it.
  * max_q: the most query tokens of one sequence (chooses the kernel; any value
  * is correct). Offsets outside the packed tensors raise the device error word
- * and are cut. */
+ * and are cut. Rows of out and lse that belong to no sequence are not written. */
 int wp_prompt_attention(wp_handle* h, void* out, float* lse, const void* q, int64_t q_ts, int64_t q_hs, const void* k,
                         int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, const int32_t* cu_q,
                         const int32_t* cu_k, int32_t num_seqs, int32_t max_q, int32_t q_tokens, int32_t k_tokens,
@@ -487,7 +487,8 @@ int wp_kv4_read(wp_handle* h, void* k, void* v, const void* pages, int32_t num_p
  * head j reads kv head j / (heads / kv_heads)), out contiguous [tokens, heads,
  * D], lse (may be NULL) [tokens, heads] fp32 log of the softmax denominator.
  * A row that sees nothing is 0 with lse -inf; what a row must not see does not
- * reach it, NaN and infinities included. max_q: the most query tokens of one
+ * reach it, NaN and infinities included; rows that belong to no sequence are
+ * not written. max_q: the most query tokens of one
  * sequence (chooses the kernel; any value is correct). workspace: DEVICE
  * scratch of at least wp_kv4_attention_workspace bytes, 16-byte aligned,
  * free for the caller again once the stream has passed the call. */

@@ -370,3 +370,20 @@ def test_nan_and_infinity_stay_in_the_cache(eng, dtype, dim):
     bad[6:, 2:] = True
     assert torch.equal(got.cpu().isnan(), bad[..., None].expand_as(got))
     assert torch.equal(got.cpu()[~bad], want.cpu()[~bad])
+
+
+def test_tensors_of_another_device_are_refused(eng):
+    """The engine's device is the cache's: everything else is refused before a
+    kernel could follow its address."""
+    b = Batch(eng, [40], 2, 64, torch.bfloat16).append_all()
+    c = b.cache
+    q = torch.randn(1, 4, 64, device="cuda").bfloat16()
+    here, eng.device = eng.device, torch.device("cuda", 1)
+    try:
+        for f in (lambda: KvCache4(eng, pages=c.pages), lambda: c.attention(q, b.table, b.lens),
+                  lambda: c.append(q[:, :2], q[:, 2:], b.table, b.lens), lambda: c.read(b.table, b.lens)):
+            with pytest.raises(RuntimeError, match="cuda:1"):
+                f()
+    finally:
+        eng.device = here
+    c.attention(q, b.table, b.lens)

@@ -203,3 +203,14 @@ def test_nan_and_infinity_among_any_logits(eng, dtype, rest, odd):
     assert bool(got.top_logprobs[:3].isnan().all())
     check(eng, x[3:], torch.tensor([5]), 2)
     assert float(want.logprob[0]) == pytest.approx(float(got.logprob[3]), rel=1e-5)
+
+
+def test_tensors_of_another_device_are_refused(eng):
+    x, t = logits(2, 100, torch.bfloat16).cuda(), torch.zeros(2, dtype=torch.int64, device="cuda")
+    here, eng.device = eng.device, torch.device("cuda", 1)
+    try:
+        with pytest.raises(RuntimeError, match="cuda:1"):
+            eng.token_logprobs(x, t)
+    finally:
+        eng.device = here
+    eng.token_logprobs(x, t)

@@ -300,3 +300,14 @@ def test_rows_computed_again_hold_nobody_up(eng):
     u = 2.0 ** -8
     big = float(v[:, :, rest].float().abs().max())
     assert bool(((a - b).abs() <= 2 * (u / 2 * b.abs() + (u / 2 + 2.0 ** -10) * big)).all())
+
+
+def test_tensors_of_another_device_are_refused(eng):
+    q, cu = torch.randn(10, 4, 64, device="cuda").bfloat16(), starts([10])
+    here, eng.device = eng.device, torch.device("cuda", 1)
+    try:
+        with pytest.raises(RuntimeError, match="cuda:1"):
+            eng.prompt_attention(q, q, q, cu)
+    finally:
+        eng.device = here
+    eng.prompt_attention(q, q, q, cu)
