@@ -58,11 +58,10 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptArgs& a, int b) {
 // the weight 0 of a key that a row must not see with that key's V, which is NaN
 // where V is not finite; rows whose result is not finite come here, so only a
 // row's own keys decide what it is. 32 keys at a time: a lane has the score of
-// one of them, then four dimensions of the output. `beat` (shared memory, or
-// null) is raised every 1024 keys, for those who wait meanwhile. The caller has
-// passed a __syncwarp since the row's first stores.
+// one of them, then four dimensions of the output. The caller has passed a
+// __syncwarp since the row's first stores.
 template <typename T>
-__device__ __forceinline__ void prompt_row(const PromptArgs& a, const PromptSeq& s, int token, int head, int* beat) {
+__device__ __forceinline__ void prompt_row(const PromptArgs& a, const PromptSeq& s, int token, int head) {
   const int lane = threadIdx.x & 31, d0 = lane * 4, kvh = head / (a.heads / a.kv_heads);
   const bool on = d0 < a.dim;
   const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(s.q0 + token) * a.q_ts + head * a.q_hs;
@@ -72,7 +71,6 @@ __device__ __forceinline__ void prompt_row(const PromptArgs& a, const PromptSeq&
   const int end = min(token + s.nk - s.nq + 1, s.nk);
 #pragma unroll 1
   for (int j0 = 0; j0 < end; j0 += 32) {
-    if (beat && lane == 0 && (j0 & 1023) == 0) atomicAdd(beat, 1);
     float x = -INFINITY;
     if (j0 + lane < end) {
       const T* kr = k + (j0 + lane) * a.k_ts;
@@ -100,7 +98,7 @@ __device__ __forceinline__ void prompt_row(const PromptArgs& a, const PromptSeq&
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] *= f;
     const int n = min(end - j0, 32);
-#pragma unroll 8
+#pragma unroll 4
     for (int t = 0; t < n; ++t) {
       const uint2 w = __ldg(reinterpret_cast<const uint2*>(v + (j0 + t) * a.v_ts));
       const float2 f0 = Elem<T>::unpack2(w.x), f1 = Elem<T>::unpack2(w.y);
@@ -307,7 +305,7 @@ __global__ void __launch_bounds__(NW * 32) prompt_small_kernel(const __grid_cons
       for (unsigned todo = __ballot_sync(~0u, bad[i]); todo;) {
         const int lead = __ffs(todo) - 1, r = r0 + warp * 16 + (lead >> 2) + 8 * i;
         todo &= ~(0xfu << (lead & ~3));
-        prompt_row<T>(a, s, r / group, kvh * group + r % group, nullptr);
+        prompt_row<T>(a, s, r / group, kvh * group + r % group);
       }
     __syncthreads();  // the next block's loads overwrite Q and the tiles
     rb += gridDim.x;
@@ -369,6 +367,15 @@ cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
 // 38 / 44. Taking the next item when the current one begins: 159, 123, 474,
 // 50.7 and 38 us; two ahead, 175 us in the first case.
 
+// Limit of the waits: rows that are computed again (prompt_row) hold the other
+// warps of the CTA up for as long as their sequence is long. The 32 rows of a
+// warp take 8 us per key with 64 dimensions and 10-12 with 128, when every warp
+// of the GPU is at it (50000 and 200000 keys). The limit is 16 polls of 4 us
+// per key of the call, and a second for the rest. (A limit that starts anew
+// while such rows come further cost every call 1-9%, in the waits' code.)
+constexpr int kPollsBase = 1 << 18, kPollsPerKey = 16;
+constexpr unsigned long long kPollNs = 4000;
+
 constexpr int kPaWarps = 12;
 constexpr int kPaThreads = kPaWarps * 32;
 constexpr int kPaProd = 8;
@@ -429,7 +436,6 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   uint64_t* o_free = kv_full + 30;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(kv_full + 32);
   volatile int* s_bad = reinterpret_cast<volatile int*>(kv_full + 33);
-  int* s_beat = reinterpret_cast<int*>(kv_full + 33) + 1;  // grows while rows are computed again
   uint64_t* next_full = kv_full + 40;  // *s_item is the next item
   uint64_t* next_empty = kv_full + 41;
   uint64_t* taken = kv_full + 42;  // a cancellation's answer is there
@@ -465,7 +471,6 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     mbar_init(next_empty, kPaWarps - 1);
     mbar_init(taken, 1);
     *s_bad = 0;
-    *s_beat = 0;
     fence_mbar_init();
   }
   if (warp == 0) tmem_alloc(s_tmem, 512);
@@ -497,20 +502,10 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   s_sum[tid] = before + incl - mine;
   __syncthreads();
 
-  // Waits of a warp and of one lane. Rows that are computed again (prompt_row)
-  // take as long as their sequence is long, so a wait goes on where its limit
-  // runs out while some row has come further since the last time.
-  auto wait_warp = [&](uint32_t bar, uint32_t parity) { return mbar_wait_warp(bar, parity, a.err, s_beat); };
+  // Waits of a warp and of one lane.
+  auto wait_warp = [&](uint32_t bar, uint32_t parity) { return mbar_wait_warp(bar, parity, a.err, a.polls); };
   auto wait_lane = [&](uint64_t* bar, uint32_t parity) {
-    for (int seen = 0; !mbar_wait_bounded(bar, parity, nullptr);) {
-      const int now = *const_cast<volatile int*>(s_beat);
-      if (now == seen) {
-        if (a.err) atomicOr(a.err, kErrWaitTimeout);
-        return false;
-      }
-      seen = now;
-    }
-    return true;
+    return mbar_wait_bounded(bar, parity, a.err, a.polls * kPollNs);
   };
   // Waits for the CTA's n-th item, a whole warp together; false past the last one.
   auto item = [&](int n, PaItem& it) {
@@ -879,7 +874,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       __syncwarp();  // a row's first stores come from another lane
       for (unsigned todo = __ballot_sync(~0u, odd && live && l == l); todo; todo &= todo - 1) {
         const int r = (warp & 3) * 32 + __ffs(todo) - 1;
-        prompt_row<T>(a, it.s, first + r / group, it.kvh * group + r % group, s_beat);
+        prompt_row<T>(a, it.s, first + r / group, it.kvh * group + r % group);
       }
     }
   }
@@ -901,8 +896,9 @@ bool prompt_map(CUtensorMap* m, int dtype, const void* base, int dim, int heads,
 }
 
 template <typename T, int DP>
-cudaError_t launch_tiles(int dtype, const PromptArgs& a, cudaStream_t stream) {
+cudaError_t launch_tiles(int dtype, PromptArgs a, cudaStream_t stream) {
   using C = PaCfg<DP>;
+  a.polls = static_cast<int>(std::min<int64_t>(kPollsBase + int64_t{kPollsPerKey} * a.k_tokens, 0x7fffffff));
   static PerDevice ready;
   if (!ready.get([] {
         return cudaFuncSetAttribute(prompt_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) ==

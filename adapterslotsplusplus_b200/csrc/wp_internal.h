@@ -316,6 +316,7 @@ struct PromptArgs {
   float scale;
   int* err;
   int pdl;
+  int polls;  // limit of the tiled kernel's waits (set by its launcher)
 };
 cudaError_t launch_prompt_attention(int dtype, const PromptArgs& a, cudaStream_t stream);
 
