@@ -345,7 +345,7 @@ cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
 // tile has its own issuer because the tensor core queues only a few products,
 // so one issuer's waits for both tiles would drain it; the issuers take turns
 // (`turn`), because two tiles whose products interleave end up with their
-// softmaxes at the same time (608 us against 494 us at the size below). The
+// softmaxes at the same time (8192 tokens, when introduced: 608 against 494 us). The
 // products of one issuer run in order, so S_i(j + 1) may follow P_i(j) V into
 // the same columns, and the arrival of S_i(j) tells that O_i holds all blocks
 // before j. P V starts on the first 64 keys' weights.
@@ -360,12 +360,13 @@ cudaError_t launch_small(const PromptArgs& a, cudaStream_t stream) {
 // still wait for an SM and takes over its item next (warp 11, which also looks
 // it up for the others). So an SM is set up once, its next item's loads run
 // while the current one ends, and no SM is left with two long items at the end.
-// Against one CTA per SM with a fixed share of the items, which every warp
-// looked up for itself (32 query / 8 kv heads of 128, device time): 4 sequences
-// of 2048 tokens 151 against 204 us, 64 of 100-400 tokens 123 / 136, one of
-// 8192 469 / 499, 16 of 1-1500 tokens 42.3 / 50.4; 64 of 256, 12 heads of 64:
-// 38 / 44. Taking the next item when the current one begins: 159, 123, 474,
-// 50.7 and 38 us; two ahead, 175 us in the first case.
+// When introduced, against one CTA per SM with a fixed share of the items, which
+// every warp looked up for itself (32 query / 8 kv heads of 128, device time): 4
+// sequences of 2048 tokens 151 against 204 us, 64 of 100-400 tokens 123 / 136,
+// one of 8192 469 / 499, 16 of 1-1500 tokens 42.3 / 50.4; 64 of 256, 12 heads of
+// 64: 38 / 44. Taking the next item when the current one begins: 159, 123, 474,
+// 50.7 and 38 us; two ahead, 175 us in the first case. Now: 145 us in the first
+// case, 437-443 for one of 8192, 38 for 64 of 256.
 
 // Limit of the waits: rows that are computed again (prompt_row) hold the other
 // warps of the CTA up for as long as their sequence is long. The 32 rows of a
@@ -385,12 +386,12 @@ constexpr int kPaKeys = 128;  // keys of a block
 template <typename T>
 constexpr float kPaLazy = Elem<T>::is_bf16 ? 8.f : 7.f;
 // Of 8 pairs of weights, those that take the FMA pipe instead of the special-
-// function unit. 32 query / 8 kv heads of 128, bf16, for 1, 2 and 3: 4 x 2048
-// tokens 158, 151 and 152 us, 64 x 100-400 tokens 126, 123 and 126, 1 x 8192
-// 478, 472 and 467 (1.17 PFLOP/s, 70% of the measured matrix rate). What bounds
-// it is the chain scores -> maximum -> weights -> products of a tile, 3000-3500
-// cycles per 128 keys against 2100 of the products alone; in long runs also the
-// power cap.
+// function unit. 32 query / 8 kv heads of 128, bf16, for 0, 1, 2 and 3: 4 x 2048
+// tokens 150, 156, 145 and 149 us, 64 x 100-400 tokens 129, 134, 131 and 135, 1
+// x 1000 25.5, 26.4, 24.8 and 25.6, 1 x 8192 472, 482, 437 and 453 (437: 1.26
+// PFLOP/s, 76% of the measured matrix rate). What bounds it is the chain scores
+// -> maximum -> weights -> products of a tile, 3300 cycles per 128 keys of two
+// tiles against 2100 of the products alone; in long runs also the power cap.
 constexpr int kPaFma = 2;
 
 template <int DP>
@@ -911,8 +912,9 @@ cudaError_t launch_tiles(int dtype, PromptArgs a, cudaStream_t stream) {
       !prompt_map(&maps.k, dtype, a.k, a.dim, a.kv_heads, a.k_tokens, a.k_ts, a.k_hs, 1, kPaKeys) ||
       !prompt_map(&maps.v, dtype, a.v, a.dim, a.kv_heads, a.k_tokens, a.v_ts, a.v_hs, 1, kPaKeys))
     return cudaErrorInvalidValue;
-  // The items are not known here: their bound (768 CTAs too many cost nothing
-  // that was measured; too few, and their items fall to CTAs that have one).
+  // The items are not known here: their bound, for offsets that ascend (768 CTAs
+  // too many cost nothing that was measured). Of offsets that do not, which
+  // raise the error bit, items past the grid are left out.
   const int64_t ctas = (static_cast<int64_t>(a.q_tokens) / (2 * tpt) + a.num_seqs) * a.kv_heads;
   if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
   return launch_after(prompt_tile_kernel<T, DP>, dim3(static_cast<unsigned>(ctas)), kPaThreads, C::SMEM, stream, a.pdl, 1, a,
@@ -921,11 +923,21 @@ cudaError_t launch_tiles(int dtype, PromptArgs a, cudaStream_t stream) {
 
 // The tiled kernel takes sequences of more than one tile of packed rows, and
 // shorter ones over long contexts, whose keys are what counts. Measured, tiled
-// against warp-level kernel (bf16): 64 sequences of 4 / 64 / 128 tokens, 12
-// heads of 64: 25.9 / 26.1 / 28.7 against 5.2 / 10.3 / 21.6 us; 16 sequences,
-// 32 query / 8 kv heads of 128, of 32 / 64 tokens (128 / 256 rows): 9.4 / 11.8
-// against 6.3 / 13.5 us; 4 tokens behind 2000 keys: 34 against 113 us, 64 rows
-// behind 500 keys: 59 against 43 us. It needs strides that a tensor map can
+// against warp-level kernel (bf16, device time), 32 query / 8 kv heads of 128,
+// 32 / 64 / 128 / 256 tokens (128 to 1024 rows):
+//   16 sequences  9.6 / 12.0 / 18.6 / 34.9 us   6.1 / 13.2 / 29.6 / 77.6
+//   64 sequences 22.0 / 30.7 / 53.2 / 109      20.8 / 42.9 / 103 / 285
+//   4 sequences   8.7 / 11.1 / 11.4 / 13.7      4.9 /  5.9 / 10.4 / 26.9
+//   1 sequence    8.6 / 11.1 / 11.1 / 12.8      4.9 /  5.8 /  8.3 / 13.5
+// 12 heads of 64, 128 / 256 / 512 tokens: 64 sequences 24.8 / 37.8 / 86.1
+// against 21.5 / 53.3 / 155, one 8.1 / 10.2 / 14.0 against 5.2 / 7.8 / 12.9. 16
+// sequences of 4 tokens (16 rows) behind 500 / 2000 keys: 14.1 / 34.1 against
+// 30.6 / 111; 64 of 4 tokens, 12 heads of 64, behind 500 / 1000: 46.1 / 77.8
+// against 35.8 / 66.9. So the crossover is that of 16 and more sequences. The
+// rule is off where the number of CTAs decides: 1 to 4 prompts of 129 to 500
+// rows lose 1 to 5 us by it, short contexts of 1000 keys without grouped heads a
+// sixth, and a few tokens of grouped heads behind 500 keys take twice as long as
+// in the other kernel. The tiled kernel needs strides that a tensor map can
 // express, and a positive scale, because its maxima are of unscaled scores.
 constexpr int64_t kTileRows = 128, kTileKeys = 1024;
 
